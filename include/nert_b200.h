@@ -64,6 +64,8 @@ extern "C" {
 #define NB2_F32 0
 #define NB2_I64 1
 #define NB2_BOOL 2
+#define NB2_F16 3  /* IEEE half: serving rows only */
+#define NB2_BF16 4 /* bfloat16: serving rows only */
 
 typedef struct nb2_device nb2_device;
 
@@ -86,6 +88,16 @@ const char* nb2_last_error(void);
 /* The process-lifetime context of GPU `ordinal` (replaces the reference's
  * process singleton CudaDevice(), src/cuda_device.cpp:98-102, one per GPU). */
 int nb2_device_open(int ordinal, nb2_device** out);
+/* A context of GPU `ordinal` whose rows launch on the caller's `stream` (a
+ * cudaStream_t; null is the legacy default stream), with a workspace and a
+ * device error word of its own: work of this context is ordered with the
+ * caller's other work on that stream, and contexts of different streams share
+ * no scratch. The stream must outlive the context. Any row takes it in place of
+ * nb2_device_open's. One host thread at a time per context. */
+int nb2_device_on_stream(int ordinal, void* stream, nb2_device** out);
+/* Waits for the stream, then frees a context from nb2_device_on_stream (null
+ * is a no-op; a context from nb2_device_open is NB2_ERR_INVALID). */
+int nb2_device_release(nb2_device* dev);
 int nb2_device_ordinal(const nb2_device* dev);
 /* The device's cudaStream_t, as an opaque pointer. */
 void* nb2_device_stream(nb2_device* dev);
@@ -276,6 +288,127 @@ int nb2_resize(nb2_device* dev, const void* x, void* y, const int64_t* in_dims, 
                const double* scales, int rank, int mode, int transform, int nearest_mode, int dtype);
 /* Cast between NB2_F32 / NB2_I64 / NB2_BOOL (float -> int64 truncates). */
 int nb2_cast(nb2_device* dev, const void* x, int from_dtype, void* y, int to_dtype, int64_t count);
+
+/* ---- serving rows: one step over a paged cache ---------------------------- */
+
+/* No counterpart in the reference, which runs whole graphs only. A step runs
+ * nb2_page_plan once, then per layer nb2_rope_append and nb2_tree_attention,
+ * and nb2_logits_process before picking tokens. Element types (`dtype`):
+ * NB2_F32, NB2_F16, NB2_BF16, the same for all floating tensors of a call
+ * unless said otherwise. Lengths, positions, slots and blocks are int32. Sizes
+ * that live on the device (lengths, offsets, block ids, token ids) cannot be
+ * checked by the host: a value out of range makes the row skip what it would
+ * address and record a device error (NB2_ERR_DEVICE at the next
+ * synchronisation); no row reads or writes out of range.
+ *
+ * Cache: block b, place p, key/value head h at b*block_stride + p*place_stride
+ * + h*head_stride elements, its head_dim values contiguous. The token at place
+ * p of request r (p = 0 .. total-1) sits in block table[r*table_stride +
+ * p/block_size] at place p % block_size; its slot is block*block_size + place. */
+
+/* Block tables, slots, positions and tree masks of one step, from the lengths.
+ * Request r has seq_lens[r] cached tokens and adds new_lens[r]. Blocks past
+ * ceil(seq_lens/block_size) are taken in request order from free_blocks,
+ * starting at free_head[0] (null: 0), and written to the table (in place).
+ * Token t of `tokens` is the (t - token_offsets[r])-th new one of request r:
+ *   new_total[r] = seq_lens[r] + new_lens[r];  token_offsets[batch + 1];
+ *   slots[t] (-1: no block), positions[t] = seq_lens[r] + depth, where depth is
+ *   its index, or with `parents` the number of its ancestors;
+ *   tree_mask[t*mask_words + j/32] bit j%32: new token j is t or an ancestor.
+ * parents[t]: index of the parent among the request's new tokens, below its
+ * own, or negative for a child of the cached text; null means a chain, and
+ * then mask_words must be 0. free_head_out[0] = free_head + blocks taken.
+ * Tokens past token_offsets[batch] get slot -1, position 0 and an empty mask.
+ * Device errors: a negative length, more new tokens than `tokens` or (with
+ * parents) than 32*mask_words, a free list or table row that is too short, a
+ * parent not below its own index. batch <= 8192, mask_words <= 32. */
+typedef struct nb2_page_plan_geom {
+    int64_t batch, tokens;
+    int64_t block_size, table_blocks, table_stride, free_blocks;
+    int64_t mask_words;
+} nb2_page_plan_geom;
+int nb2_page_plan(nb2_device* dev, const nb2_page_plan_geom* g, const int32_t* seq_lens, const int32_t* new_lens,
+                  const int32_t* free_blocks, const int32_t* free_head, const int32_t* parents, int32_t* block_table,
+                  int32_t* new_total, int32_t* token_offsets, int32_t* free_head_out, int32_t* slots,
+                  int32_t* positions, int32_t* tree_mask);
+
+/* Rotary positions with up to 8 axes, and the cache write. Frequency f of
+ * rot_dim/2 turns the pair (x1, x2) of a head by the angle of position
+ * p = positions[axis_of[f]*axis_stride + t]:  y1 = x1*c - x2*s, y2 = x2*c + x1*s,
+ * c = table[p*rot_dim + f], s = table[p*rot_dim + rot_dim/2 + f] (fp32). The
+ * pair is elements (f, f + rot_dim/2), or (2f, 2f + 1) when interleaved; the
+ * rest of the head is copied. q [tokens, q_heads, head_dim] goes to q_out; k to
+ * k_out (may be null) and, with k_cache, to slot slots[t]; v is copied to
+ * v_cache at the same slot (a negative slot is skipped). q_out may be q and
+ * k_out k (same strides). head_dim and rot_dim even, head_dim <= 512. A token
+ * or cache stride is in elements. */
+typedef struct nb2_rope_geom {
+    int64_t tokens, q_heads, kv_heads, head_dim, rot_dim;
+    int64_t q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride;
+    int64_t qo_stride, qo_head_stride, ko_stride, ko_head_stride;
+    int64_t table_len, axis_stride;
+    int64_t block_size, num_blocks;
+    int64_t kc_block_stride, kc_place_stride, kc_head_stride;
+    int64_t vc_block_stride, vc_place_stride, vc_head_stride;
+    int32_t axes, interleaved, dtype, reserved;
+    uint8_t axis_of[256];
+} nb2_rope_geom;
+int nb2_rope_append(nb2_device* dev, const nb2_rope_geom* g, const void* q, const void* k, const void* v,
+                    const float* table, const int32_t* positions, const int32_t* slots, void* q_out, void* k_out,
+                    void* k_cache, void* v_cache);
+
+/* Attention of each request's new tokens over its cached tokens and over the
+ * new tokens that its tree allows (their keys and values already in the
+ * cache). Request r has total_lens[r] places, the last n = token_offsets[r+1] -
+ * token_offsets[r] of them new; new token i sees every older place, and new
+ * token j where bit j of its tree_mask row is set (mask_words 0 and null
+ * tree_mask: j <= i). out[t, h] = sum_j softmax_j(scale q.k_j) v_j with query head
+ * h reading key/value head h / (q_heads/kv_heads); lse[t, h] (may be null) =
+ * log sum_j exp(scale q.k_j), fp32. A token that sees nothing has out 0 and lse
+ * -inf, as have tokens past token_offsets[batch]. Scores, softmax and sums in
+ * fp32; NB2_F32 products by the 3xTF32 split. max_new bounds the new tokens of
+ * a request (more are a device error, and such a request's tokens get out 0).
+ * head_dim a multiple of 8 up to 256, every stride and pointer 16-byte aligned,
+ * batch <= 8192, kv_heads <= 65535. Scratch comes from the device workspace. */
+typedef struct nb2_tree_attn_geom {
+    int64_t batch, tokens, q_heads, kv_heads, head_dim, max_new;
+    int64_t q_stride, q_head_stride, o_stride, o_head_stride;
+    int64_t block_size, num_blocks, table_blocks, table_stride;
+    int64_t kc_block_stride, kc_place_stride, kc_head_stride;
+    int64_t vc_block_stride, vc_place_stride, vc_head_stride;
+    int64_t mask_words;
+    float scale;
+    int32_t dtype;
+} nb2_tree_attn_geom;
+int nb2_tree_attention(nb2_device* dev, const nb2_tree_attn_geom* g, const void* q, const void* k_cache,
+                       const void* v_cache, const int32_t* block_table, const int32_t* total_lens,
+                       const int32_t* token_offsets, const int32_t* tree_mask, void* out, float* lse);
+
+/* Logit rules: for row i with request r = row_request[i] (null: r = i) and
+ * token v, c = how often v is in the request's output list, and seen = c > 0 or
+ * v in its prompt list, in fp32:
+ *   x = logits[i, v];  seen: x = x > 0 ? x / repetition[r] : x * repetition[r];
+ *   x -= frequency[r] * c + (c > 0 ? presence[r] : 0);  x += bias[r, v];
+ *   x = -inf where grammar row grammar_rows[i] (null: i; negative: no rule) has
+ *   bit v%32 of word v/32 clear, whatever x was (NaN too).
+ * Lists are ragged: ids [offsets[r], offsets[r+1]); an id that comes twice in
+ * a bias list takes its last value. Any of the lists with its offsets, the
+ * factors (1, 0 and 0) and the grammar may be null. out may be logits when the
+ * types and strides agree. in_dtype and out_dtype NB2_F32, NB2_F16 or NB2_BF16.
+ * `requests` bounds r, `grammar_count` the grammar's rows. */
+typedef struct nb2_logits_geom {
+    int64_t rows, vocab, requests;
+    int64_t in_stride, out_stride;
+    int64_t grammar_count, grammar_stride; /* rows; words per row */
+    int64_t prompt_count, output_count, bias_count; /* ids held by each list */
+    int32_t in_dtype, out_dtype;
+} nb2_logits_geom;
+int nb2_logits_process(nb2_device* dev, const nb2_logits_geom* g, const void* logits, void* out,
+                       const int32_t* row_request, const int32_t* prompt_ids, const int32_t* prompt_offsets,
+                       const int32_t* output_ids, const int32_t* output_offsets, const float* repetition,
+                       const float* presence, const float* frequency, const int32_t* bias_ids,
+                       const float* bias_values, const int32_t* bias_offsets, const int32_t* grammar,
+                       const int32_t* grammar_rows);
 
 /* ---- engine: whole graphs ------------------------------------------------ */
 

@@ -17,7 +17,7 @@ DEVICE_LIB_PATH = os.path.join(HERE, "lib", "libnert_b200_device.so")
 OK, ERR_INVALID, ERR_CUDA, ERR_DEVICE, ERR_UNSUPPORTED, ERR_NOMEM = 0, -1, -2, -3, -4, -5
 PREC_3XTF32, PREC_1XTF32 = 0, 1
 ACT_NONE, ACT_RELU, ACT_SILU, ACT_SIGMOID = 0, 1, 2, 3
-F32, I64, BOOL = 0, 1, 2
+F32, I64, BOOL, F16, BF16 = 0, 1, 2, 3, 4
 
 c_i64p = ctypes.POINTER(ctypes.c_int64)
 vp = ctypes.c_void_p
@@ -41,10 +41,41 @@ class ConvTGeom(ctypes.Structure):
         "pad_bottom", "pad_right", "dil_h", "dil_w", "out_pad_h", "out_pad_w", "group")]
 
 
+class PagePlanGeom(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in (
+        "batch", "tokens", "block_size", "table_blocks", "table_stride", "free_blocks", "mask_words")]
+
+
+class RopeGeom(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in (
+        "tokens", "q_heads", "kv_heads", "head_dim", "rot_dim", "q_stride", "q_head_stride", "k_stride",
+        "k_head_stride", "v_stride", "v_head_stride", "qo_stride", "qo_head_stride", "ko_stride", "ko_head_stride",
+        "table_len", "axis_stride", "block_size", "num_blocks", "kc_block_stride", "kc_place_stride",
+        "kc_head_stride", "vc_block_stride", "vc_place_stride", "vc_head_stride")] + [
+        (n, ctypes.c_int32) for n in ("axes", "interleaved", "dtype", "reserved")] + [
+        ("axis_of", ctypes.c_uint8 * 256)]
+
+
+class TreeAttnGeom(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in (
+        "batch", "tokens", "q_heads", "kv_heads", "head_dim", "max_new", "q_stride", "q_head_stride", "o_stride",
+        "o_head_stride", "block_size", "num_blocks", "table_blocks", "table_stride", "kc_block_stride",
+        "kc_place_stride", "kc_head_stride", "vc_block_stride", "vc_place_stride", "vc_head_stride",
+        "mask_words")] + [("scale", ctypes.c_float), ("dtype", ctypes.c_int32)]
+
+
+class LogitsGeom(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in (
+        "rows", "vocab", "requests", "in_stride", "out_stride", "grammar_count", "grammar_stride", "prompt_count",
+        "output_count", "bias_count")] + [("in_dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32)]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     "nb2_last_error": (ctypes.c_char_p, []),
     "nb2_device_open": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(vp)]),
+    "nb2_device_on_stream": (ctypes.c_int, [ctypes.c_int, vp, ctypes.POINTER(vp)]),
+    "nb2_device_release": (ctypes.c_int, [vp]),
     "nb2_device_ordinal": (ctypes.c_int, [vp]),
     "nb2_device_stream": (vp, [vp]),
     "nb2_device_set_precision": (ctypes.c_int, [vp, ctypes.c_int]),
@@ -97,6 +128,10 @@ _SIGS = {
     "nb2_resize": (ctypes.c_int, [vp, vp, vp, c_i64p, c_i64p, ctypes.POINTER(ctypes.c_double), ctypes.c_int,
                                   ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
     "nb2_cast": (ctypes.c_int, [vp, vp, ctypes.c_int, vp, ctypes.c_int, ctypes.c_int64]),
+    "nb2_page_plan": (ctypes.c_int, [vp, ctypes.POINTER(PagePlanGeom)] + [vp] * 12),
+    "nb2_rope_append": (ctypes.c_int, [vp, ctypes.POINTER(RopeGeom)] + [vp] * 10),
+    "nb2_tree_attention": (ctypes.c_int, [vp, ctypes.POINTER(TreeAttnGeom)] + [vp] * 9),
+    "nb2_logits_process": (ctypes.c_int, [vp, ctypes.POINTER(LogitsGeom)] + [vp] * 15),
 }
 
 _lib = None

@@ -150,6 +150,21 @@ int nb2_device_open(int ordinal, nb2_device** out) {
     });
 }
 
+int nb2_device_on_stream(int ordinal, void* stream, nb2_device** out) {
+    return guard([&] {
+        need(out != nullptr, "null output pointer");
+        *out = device_on_stream(ordinal, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int nb2_device_release(nb2_device* dev) {
+    return guard([&] {
+        if (dev != nullptr) {
+            release_device(dev);
+        }
+    });
+}
+
 int nb2_device_ordinal(const nb2_device* dev) { return dev ? dev->ordinal : -1; }
 
 void* nb2_device_stream(nb2_device* dev) { return dev ? static_cast<void*>(dev->stream) : nullptr; }
@@ -202,7 +217,10 @@ int nb2_device_synchronize(nb2_device* dev) {
         const int code = dev->take_device_error();
         if (code != 0) {
             fail(kStatusDevice, "a kernel reported device error " + std::to_string(code) +
-                                    (code == 1 ? " (bounded wait expired)" : code == 2 ? " (index out of range)" : ""));
+                                    (code == 1   ? " (bounded wait expired)"
+                                     : code == 2 ? " (index out of range)"
+                                     : code == 3 ? " (no free block for a cached token)"
+                                                 : ""));
         }
     });
 }

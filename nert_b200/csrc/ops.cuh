@@ -27,7 +27,7 @@ enum UnaryOp : int {
 enum BinaryOp : int { kBAdd = 0, kBSub = 1, kBMul = 2, kBDiv = 3, kBPow = 4 };
 
 // dtype codes shared with the C ABI
-enum Dtype : int { kF32 = 0, kI64 = 1, kBool = 2 };
+enum Dtype : int { kF32 = 0, kI64 = 1, kBool = 2, kF16 = 3, kBF16 = 4 };
 
 constexpr int kMaxRank = 8;
 

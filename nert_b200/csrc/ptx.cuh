@@ -13,7 +13,8 @@ namespace nb2 {
 enum DeviceError : int {
     kDevOk = 0,
     kDevWaitTimeout = 1,   // an mbarrier wait ran past its bound
-    kDevIndexOutOfRange = 2, // a Gather/TopK index outside the axis
+    kDevIndexOutOfRange = 2, // an index (Gather, TopK, a length, slot, block or token id) outside its range
+    kDevNoBlock = 3,         // a page plan's free list or table row is too short
 };
 
 // About one second at the B200's SM clock. Waits on the pipeline take their

@@ -84,6 +84,12 @@ struct nb2_device {
     int capturing = 0; // inside a CUDA-graph capture: the workspace may not grow
     int no_grow = 0;   // inside a call that must not allocate: contractions never split K
     int num_sms = 148;
+    bool callers_stream = false; // made by nb2_device_on_stream: the stream is not ours
+    // Zeroed words that kernels count arrivals in and set back to zero before
+    // they end (grow-only; outgrown ones are kept, as split_ws's are).
+    uint32_t* ticket_ws = nullptr;
+    size_t ticket_count = 0;
+    std::vector<void*> retired_tickets;
     // clock64 ticks after which a tensor-core kernel's mbarrier wait gives
     // up, records a device error and unwinds (default about one second)
     long long wait_bound;
@@ -112,10 +118,18 @@ struct nb2_device {
     // CUDA-graph capture (the caller then runs without splitting K). Growing
     // synchronises the stream first and retires (keeps) the old buffer.
     void* split_scratch(size_t bytes);
+    // At least `n` zeroed ticket words for kernels on this device's stream.
+    uint32_t* tickets(size_t n);
+    // Whether the stream is inside a CUDA-graph capture (the engine's or a
+    // caller's own), where nothing may be allocated or waited for.
+    bool in_capture() const;
     // Reads and clears the device error word (synchronises the stream).
     int take_device_error();
 };
 
 namespace nb2 {
 nb2_device* device(int ordinal);
+// A new context of the GPU on the caller's stream, and its end.
+nb2_device* device_on_stream(int ordinal, cudaStream_t stream);
+void release_device(nb2_device* dev);
 } // namespace nb2
