@@ -1,127 +1,782 @@
 // Attention of each request's new tokens over its paged cache and over the
 // new tokens that its tree allows.
 //
-// One CTA per (new token, query head) walks the request's places in tiles of
-// 128: a thread scores one place, the tile's maximum and sum update a running
-// softmax, and every thread then adds the tile's values to its elements of the
-// output. A place that the token does not see, or whose block id is out of
-// range, has weight zero and is never read.
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(s_j - m),  s_j = scale log2(e) q.k_j
+//
+// in one pass over the cache with the running maximum m and sum of each row.
+// A row is one query head of one new token; the rows of a request that share a
+// key/value head (its n tokens times the group of q_heads/kv_heads) are one
+// matrix, cut into blocks of 16 WR rows, so a key or value read once from HBM serves
+// them all. Few rows: bound by HBM (4 flops a row for each element of the cache);
+// many: by the tensor cores.
+//
+// Work split. The lengths are on the device, so the split is made there: an item is (request,
+// key/value head, row block), its units the request's tiles of KT places, and the units of all
+// items, in order, are cut into equal spans, one a CTA (a grid that fits the GPU at once), so every
+// CTA reads the same number of tiles whatever the lengths. An item inside one span is finished by
+// its CTA; of one that is cut, each CTA leaves (O, m, sum) in its own slot (a span cuts at most its
+// first and its last item: two slots a CTA) and the CTA that arrives last adds the pieces in span
+// order, so the result does not depend on which one that is.
+//
+// Within a CTA, WR x WK warps: row group x part of the tile's places. The warps of a row group run
+// the softmax on their own places and join at the end of the item. Tiles come by 16-byte cp.async
+// through a ring of NS stages, the addresses of a tile's rows looked up in the block table one tile
+// ahead of its copies.
 
 #include "serving.cuh"
+
+#include <type_traits>
 
 namespace nb2 {
 
 namespace {
 
-constexpr int kSimpleThreads = 128;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 
-template <typename T>
-__global__ void __launch_bounds__(kSimpleThreads) tree_attn_kernel(TreeAttnArgs a) {
-    const nb2_tree_attn_geom& g = a.g;
-    __shared__ float q[256], p[kSimpleThreads], red[kSimpleThreads / 32];
-    __shared__ int64_t at[kSimpleThreads];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t t = blockIdx.x;
-    const int64_t h = blockIdx.y, kvh = h / (g.q_heads / g.kv_heads);
-    const int D = static_cast<int>(g.head_dim);
-    T* out = static_cast<T*>(a.out) + t * g.o_stride + h * g.o_head_stride;
-    int lo = 0, hi = static_cast<int>(g.batch); // request of token t
-    bool bad = false;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        (a.offsets[mid] <= t ? lo : hi) = mid;
+// ---- the split of the work ----------------------------------------------------
+
+struct Request {
+    int64_t first;  // its first token
+    int n, total;   // new tokens, places (0 where the lengths cannot be right)
+    int row_blocks; // blocks of its n * group rows
+    int tiles;      // tiles of its places, at least one so that rows without places are written
+    bool bad;
+    __device__ __forceinline__ int64_t units(int64_t kv_heads) const {
+        return static_cast<int64_t>(row_blocks) * kv_heads * tiles;
     }
-    const int64_t first = g.batch > 0 ? a.offsets[lo] : 0, end = g.batch > 0 ? a.offsets[lo + 1] : 0;
-    const int64_t n = end - first, i = t - first;
-    int64_t total = i >= 0 && i < n ? a.total[lo] : 0;
-    if (total > 0 && (total < n || total > g.table_blocks * g.block_size || n > g.max_new)) {
-        bad = true;
-        total = 0;
+};
+
+template <int RT, int KT>
+__device__ __forceinline__ Request request_at(const TreeAttnArgs& a, int r, int group) {
+    Request q{};
+    const int64_t lo = a.offsets[r], hi = a.offsets[r + 1];
+    const int64_t total = a.total[r];
+    if (lo < 0 || hi < lo || hi > a.g.tokens) {
+        q.bad = true;
+        return q;
     }
-    const int64_t old = total - n;
-    for (int d = tid; d < D; d += kSimpleThreads) {
-        q[d] = to_f32(static_cast<const T*>(a.q)[t * g.q_stride + h * g.q_head_stride + d]);
+    q.first = lo;
+    q.n = static_cast<int>(hi - lo);
+    if (q.n == 0) {
+        return q;
+    }
+    q.bad = total < q.n || total > a.g.table_blocks * a.g.block_size || q.n > a.g.max_new;
+    q.total = q.bad ? 0 : static_cast<int>(total);
+    q.row_blocks = static_cast<int>((static_cast<int64_t>(q.n) * group + RT - 1) / RT);
+    q.tiles = max(1, (q.total + KT - 1) / KT);
+    return q;
+}
+
+// CTA whose span holds unit w, of `grid` spans [c W / grid, (c + 1) W / grid).
+__device__ __forceinline__ int cta_of(int64_t w, int64_t W, int64_t grid) {
+    return static_cast<int>(((w + 1) * grid - 1) / W);
+}
+
+template <int NT>
+__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* red) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        v += __shfl_xor_sync(0xffffffffu, v, o);
     }
     __syncthreads();
-    float m = -INFINITY, z = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int64_t j0 = 0; j0 < total; j0 += kSimpleThreads) {
-        const int64_t j = j0 + tid;
-        bool see = j < total;
-        if (see && j >= old) {
-            const int64_t k = j - old;
-            see = a.mask == nullptr ? k <= i
-                                    : k < 32 * g.mask_words && ((a.mask[t * g.mask_words + (k >> 5)] >> (k & 31)) & 1u);
-        }
-        int64_t block = -1;
-        if (see) {
-            block = a.table[lo * g.table_stride + j / g.block_size];
-            if (block < 0 || block >= g.num_blocks) {
-                bad = true;
-                see = false;
-            }
-        }
-        float s = -INFINITY;
-        if (see) {
-            const int64_t place = j % g.block_size;
-            const T* k = static_cast<const T*>(a.kc) + block * g.kc_block_stride + place * g.kc_place_stride +
-                         kvh * g.kc_head_stride;
-            s = 0.0f;
-            for (int d = 0; d < D; ++d) {
-                s += q[d] * to_f32(k[d]);
-            }
-            s *= g.scale;
-            at[tid] = block * g.vc_block_stride + place * g.vc_place_stride + kvh * g.vc_head_stride;
-        } else {
-            at[tid] = -1;
-        }
-        float top = s;
+    if ((threadIdx.x & 31) == 0) {
+        red[threadIdx.x >> 5] = v;
+    }
+    __syncthreads();
+    int64_t s = 0;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int w = 0; w < NT / 32; ++w) {
+        s += red[w];
+    }
+    return s;
+}
+
+// ---- instructions ----------------------------------------------------------------
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+    const int n = live ? 16 : 0; // 0: sixteen zero bytes
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same_v<T, __half>) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    } else {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+}
+
+__device__ __forceinline__ void mma_tf32_8(float (&d)[4], const float (&a)[4], float b0, float b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])),
+                   "r"(__float_as_uint(a[3])), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (std::is_same_v<T, __half>) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// ---- the kernel -----------------------------------------------------------------
+
+template <typename T, int DP, int WR, int WK>
+struct Shape {
+    static constexpr bool kF32Type = sizeof(T) == 4;
+    static constexpr int kWarps = WR * WK, kThreads = 32 * kWarps;
+    static constexpr int RT = 16 * WR;                    // rows of a block
+    static constexpr int KT = kF32Type ? 32 : 64;         // places of a tile
+    static constexpr int KW = KT / WK;                    // places of a warp
+    static constexpr int kChunks = DP * sizeof(T) / 16;   // 16-byte chunks of a row
+    static constexpr int kRow = DP * sizeof(T) + (kF32Type ? 16 : 0); // bytes of a row in shared memory
+    static constexpr int kTile = KT * kRow;
+    // stages of the ring: what fits beside Q
+    static constexpr int NS = DP == 64 ? 4 : DP == 128 || (WR == 1 && !kF32Type) ? 3 : 2;
+    static constexpr int kRing = NS * 2 * kTile;
+    static constexpr int kQ = RT * kRow * (kF32Type ? 2 : 1);
+    static constexpr int kJoin = WK * RT * DP * 4;        // the warps' sums, over the ring
+    static constexpr int kSmem = (kRing > kJoin ? kRing : kJoin) + kQ + 1024;
+};
+
+template <typename T, int DP, int WR, int WK>
+__global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(TreeAttnArgs a, int group, float* part_o,
+                                                                 float2* part_ml, uint32_t* tickets) {
+    using S = Shape<T, DP, WR, WK>;
+    constexpr int NT = S::kThreads, RT = S::RT, KT = S::KT, KW = S::KW, NS = S::NS;
+    constexpr int NB = KW / 8; // 8-place column blocks of a warp's scores
+    extern __shared__ __align__(1024) uint8_t attn_dyn[];
+    uint8_t* ring = attn_dyn;
+    uint8_t* qs = attn_dyn + (S::kRing > S::kJoin ? S::kRing : S::kJoin);
+    __shared__ int64_t red[NT / 32];
+    __shared__ int64_t k_at[NS][KT], v_at[NS][KT]; // element offsets of a tile's rows, -1: no such place
+    __shared__ int holes[NS][KT / 32];             // a place inside total has no block
+    __shared__ unsigned long long odd_keys;        // places of the tile whose values are not finite
+    __shared__ float2 warp_ml[WK][RT];
+    __shared__ int64_t start_unit;
+    __shared__ int start_request, is_last;
+
+    const nb2_tree_attn_geom& g = a.g;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int wr = warp / WK, wk = warp % WK;
+    const int gq = lane >> 2, cq = lane & 3;
+    const int B = static_cast<int>(g.batch);
+    const int64_t cta = blockIdx.x;
+    const int D = static_cast<int>(g.head_dim);
+    const float scale2 = g.scale * kLog2e;
+    bool bad = false;
+
+    // ---- this CTA's span
+    int64_t sum = 0;
+    for (int r = tid; r < B; r += NT) {
+        const Request q = request_at<RT, KT>(a, r, group);
+        bad |= q.bad;
+        sum += q.units(g.kv_heads);
+    }
+    const int64_t W = block_sum<NT>(sum, red);
+    // tokens that belong to no request
+    {
+        const int64_t lo = B > 0 ? a.offsets[0] : 0, hi = B > 0 ? a.offsets[B] : 0;
+        const int64_t before = min(max(lo, int64_t{0}), g.tokens), after = min(max(hi, before), g.tokens);
+        const int64_t spare = (before + g.tokens - after) * g.q_heads;
+        for (int64_t i = cta * NT + tid; i < spare; i += static_cast<int64_t>(gridDim.x) * NT) {
+            int64_t t = i / g.q_heads;
+            const int64_t h = i - t * g.q_heads;
+            t = t < before ? t : t - before + after;
+            T* row = static_cast<T*>(a.out) + t * g.o_stride + h * g.o_head_stride;
+            for (int d = 0; d < D; ++d) {
+                row[d] = from_f32<T>(0.0f);
+            }
+            if (a.lse != nullptr) {
+                a.lse[t * g.q_heads + h] = -INFINITY;
+            }
         }
-        if (lane == 0) {
-            red[warp] = top;
+    }
+    const int64_t grid = min(static_cast<int64_t>(gridDim.x), W); // no span is empty
+    const int64_t w0 = cta < grid ? cta * W / grid : 0, w1 = cta < grid ? (cta + 1) * W / grid : 0;
+    if (w0 < w1) {
+        int64_t base = 0;
+        for (int c = 0; c < B; c += NT) { // the request that holds unit w0
+            const int64_t u = c + tid < B ? request_at<RT, KT>(a, c + tid, group).units(g.kv_heads) : 0;
+            int64_t inc = u;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t up = __shfl_up_sync(0xffffffffu, inc, o);
+                inc += lane >= o ? up : 0;
+            }
+            __syncthreads();
+            if (lane == 31) {
+                red[warp] = inc;
+            }
+            __syncthreads();
+            int64_t all = 0;
+#pragma unroll
+            for (int w = 0; w < NT / 32; ++w) {
+                inc += w < warp ? red[w] : 0;
+                all += red[w];
+            }
+            inc += base;
+            if (inc - u <= w0 && w0 < inc) {
+                start_request = c + tid;
+                start_unit = inc - u;
+            }
+            base += all;
+            if (base > w0) {
+                break;
+            }
         }
         __syncthreads();
-        top = m;
-        for (int w = 0; w < kSimpleThreads / 32; ++w) {
-            top = fmaxf(top, red[w]);
+    }
+
+    int r = w0 < w1 ? start_request : 0;
+    int64_t r_unit = w0 < w1 ? start_unit : 0; // first unit of request r
+    Request rq{};
+    if (w0 < w1) {
+        rq = request_at<RT, KT>(a, r, group);
+    }
+    for (int64_t w = w0; w < w1;) {
+        while (w >= r_unit + rq.units(g.kv_heads)) {
+            r_unit += rq.units(g.kv_heads);
+            rq = request_at<RT, KT>(a, ++r, group);
         }
-        const float ref = top == -INFINITY ? 0.0f : top;
-        p[tid] = expf(s - ref);
+        // ---- the item and this CTA's tiles of it
+        const int64_t item = (w - r_unit) / rq.tiles;
+        const int64_t item_w0 = r_unit + item * rq.tiles, item_w1 = item_w0 + rq.tiles;
+        const int64_t kvh = item / rq.row_blocks;
+        const int rb = static_cast<int>(item - kvh * rq.row_blocks);
+        const int t_begin = static_cast<int>(w - item_w0);
+        const int t_end = static_cast<int>(min(w1, item_w1) - item_w0);
+        const int rows = min(RT, rq.n * group - rb * RT);
+        const int old = rq.total - rq.n; // -n where the lengths are wrong: then total is 0 and no place is seen
+        const int32_t* table = a.table + r * g.table_stride;
+
+        __syncthreads(); // the last item's use of shared memory is over
+        // ---- Q rows into shared memory, zero past the block's rows and head_dim
+        for (int i = tid; i < RT * S::kChunks; i += NT) {
+            const int row = i / S::kChunks, ch = i - row * S::kChunks;
+            constexpr int E = 16 / sizeof(T);
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (row < rows && ch * E < D) {
+                const int rho = rb * RT + row, tok = rho / group;
+                const int64_t h = kvh * group + (rho - tok * group);
+                x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (rq.first + tok) * g.q_stride +
+                                                    h * g.q_head_stride + ch * E);
+            }
+            if constexpr (S::kF32Type) { // as tf32 high and low parts
+                float f[4] = {__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w)};
+                float hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    hi[e] = to_tf32(f[e]);
+                    lo[e] = to_tf32(f[e] - hi[e]);
+                }
+                *reinterpret_cast<float4*>(qs + row * S::kRow + ch * 16) = make_float4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<float4*>(qs + (RT + row) * S::kRow + ch * 16) = make_float4(lo[0], lo[1], lo[2], lo[3]);
+            } else {
+                *reinterpret_cast<uint4*>(qs + row * S::kRow + ((ch ^ (row & 7)) << 4)) = x;
+            }
+        }
+        // rows of this thread's fragments: the token and its mask row
+        int tok0, tok1;
+        const uint32_t *mask0 = nullptr, *mask1 = nullptr;
+        {
+            const int l0 = wr * 16 + gq, l1 = l0 + 8;
+            tok0 = l0 < rows ? (rb * RT + l0) / group : -1;
+            tok1 = l1 < rows ? (rb * RT + l1) / group : -1;
+            if (a.mask != nullptr) {
+                mask0 = a.mask + (rq.first + max(tok0, 0)) * g.mask_words;
+                mask1 = a.mask + (rq.first + max(tok1, 0)) * g.mask_words;
+            }
+        }
+
+        // block of place j of this request, for the row addresses of a tile; -1: none
+        auto look_up = [&](int tile) -> int {
+            const int j = tile * KT + tid;
+            if (tid >= KT || tile >= t_end || j >= rq.total) {
+                return -2;
+            }
+            return table[j / static_cast<int>(g.block_size)];
+        };
+        auto place_rows = [&](int tile, int block) {
+            if (tid < KT) {
+                const int st = (tile - t_begin) % NS;
+                int64_t ka = -1, va = -1;
+                const bool hole = block != -2 && (block < 0 || block >= g.num_blocks);
+                const uint32_t any = __ballot_sync(0xffffffffu, hole);
+                if (lane == 0) {
+                    holes[st][warp] = any != 0;
+                }
+                bad |= hole;
+                if (block >= 0 && block < g.num_blocks) {
+                    const int64_t p = (tile * KT + tid) % static_cast<int>(g.block_size);
+                    ka = block * g.kc_block_stride + p * g.kc_place_stride + kvh * g.kc_head_stride;
+                    va = block * g.vc_block_stride + p * g.vc_place_stride + kvh * g.vc_head_stride;
+                }
+                k_at[st][tid] = ka;
+                v_at[st][tid] = va;
+            }
+        };
+        auto copy_tile = [&](int tile) {
+            if (tile < t_end) {
+                const int st = (tile - t_begin) % NS;
+                const uint32_t dst = smem_u32(ring + st * 2 * S::kTile);
+                constexpr int kPer = NT / S::kChunks > 0 ? NT / S::kChunks : 1; // rows of one pass
+                static_assert(NT % S::kChunks == 0 && KT % kPer == 0, "the threads cover whole rows");
+                const int ch = tid % S::kChunks, row0 = tid / S::kChunks;
+                const bool in = ch * static_cast<int>(16 / sizeof(T)) < D;
+                const T* kc = static_cast<const T*>(a.kc) + ch * (16 / sizeof(T));
+                const T* vc = static_cast<const T*>(a.vc) + ch * (16 / sizeof(T));
+#pragma unroll
+                for (int i = 0; i < KT / kPer; ++i) {
+                    const int row = row0 + i * kPer;
+                    const int64_t ka = k_at[st][row], va = v_at[st][row];
+                    const uint32_t off = row * S::kRow + (S::kF32Type ? ch * 16 : ((ch ^ (row & 7)) << 4));
+                    const bool live = in && ka >= 0;
+                    cp_async16(dst + off, kc + (live ? ka : 0), live);
+                    cp_async16(dst + S::kTile + off, vc + (live ? va : 0), live);
+                }
+            }
+            cp_commit();
+        };
+
+#pragma unroll
+        for (int i = 0; i < NS - 1; ++i) {
+            place_rows(t_begin + i, look_up(t_begin + i));
+        }
         __syncthreads();
-        const float keep = expf(m - ref);
-        m = top;
-        z *= keep;
-        o0 *= keep;
-        o1 *= keep;
-        for (int k = 0; k < kSimpleThreads; ++k) {
-            if (at[k] < 0) {
+#pragma unroll
+        for (int i = 0; i < NS - 1; ++i) {
+            copy_tile(t_begin + i);
+        }
+
+        uint32_t qf[S::kF32Type ? 1 : DP / 16][4];
+        if constexpr (!S::kF32Type) {
+            const int row = wr * 16 + (lane & 15);
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+                ldsm4(qf[k], smem_u32(qs + row * S::kRow + (((2 * k + (lane >> 4)) ^ (row & 7)) << 4)));
+            }
+        }
+        float o[DP / 8][4];
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i) {
+            o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        }
+        float m0 = -INFINITY, m1 = -INFINITY, z0 = 0.0f, z1 = 0.0f; // of rows gq and gq + 8, this thread's columns
+
+        for (int tile = t_begin; tile < t_end; ++tile) {
+            const int st = (tile - t_begin) % NS;
+            const int next = look_up(tile + NS - 1);
+            cp_wait<NS - 2>();
+            __syncthreads(); // the tile has landed; the stage before it is free
+            if (tid == 0) {
+                odd_keys = 0;
+            }
+            const int j0 = tile * KT;
+            const bool plain = j0 + KT <= old && holes[st][0] == 0 && holes[st][KT / 32 - 1] == 0;
+            uint8_t* kt = ring + st * 2 * S::kTile;
+            uint8_t* vt = kt + S::kTile;
+            if (!plain) {
+                // Values that are not finite would reach the rows that do not
+                // see them as 0 * inf: taken out of the tile here, added for the rows that do below.
+                __syncthreads();
+                for (int i = tid; i < KT * (S::kRow / 16); i += NT) {
+                    const int row = i / (S::kRow / 16);
+                    const T* e = reinterpret_cast<const T*>(vt + row * S::kRow + (i - row * (S::kRow / 16)) * 16);
+                    if (S::kF32Type && (i - row * (S::kRow / 16)) >= S::kChunks) {
+                        continue; // the padding of a row
+                    }
+                    bool odd = false;
+#pragma unroll
+                    for (int x = 0; x < static_cast<int>(16 / sizeof(T)); ++x) {
+                        odd |= !isfinite(to_f32(e[x]));
+                    }
+                    if (odd) {
+                        atomicOr(&odd_keys, 1ull << row);
+                    }
+                }
+                __syncthreads();
+                if (odd_keys != 0) {
+                    for (int i = tid; i < KT * (S::kRow / 16); i += NT) {
+                        const int row = i / (S::kRow / 16);
+                        if ((odd_keys >> row) & 1) {
+                            *reinterpret_cast<uint4*>(vt + i * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                    __syncthreads();
+                }
+            }
+            // ---- scores of this warp's places
+            float s[NB][4];
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
+            }
+            if constexpr (S::kF32Type) {
+#pragma unroll 4
+                for (int k = 0; k < DP / 16; ++k) {
+                    // dims 16k + 4c .. + 3 of a thread: the contraction's order is free, so k index c and
+                    // c + 4 of the two steps are dims 4c, 4c + 1 and 4c + 2, 4c + 3
+                    const uint8_t* qa = qs + (wr * 16 + gq) * S::kRow + (4 * k + cq) * 16;
+                    const float4 h0 = *reinterpret_cast<const float4*>(qa);
+                    const float4 h1 = *reinterpret_cast<const float4*>(qa + 8 * S::kRow);
+                    const float4 l0 = *reinterpret_cast<const float4*>(qa + RT * S::kRow);
+                    const float4 l1 = *reinterpret_cast<const float4*>(qa + (RT + 8) * S::kRow);
+                    const float ah0[4] = {h0.x, h1.x, h0.y, h1.y}, ah1[4] = {h0.z, h1.z, h0.w, h1.w};
+                    const float al0[4] = {l0.x, l1.x, l0.y, l1.y}, al1[4] = {l0.z, l1.z, l0.w, l1.w};
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        const float4 x = *reinterpret_cast<const float4*>(kt + (wk * KW + nb * 8 + gq) * S::kRow +
+                                                                          (4 * k + cq) * 16);
+                        const float bx = to_tf32(x.x), by = to_tf32(x.y), bz = to_tf32(x.z), bw = to_tf32(x.w);
+                        mma_tf32_8(s[nb], al0, bx, by);
+                        mma_tf32_8(s[nb], ah0, to_tf32(x.x - bx), to_tf32(x.y - by));
+                        mma_tf32_8(s[nb], ah0, bx, by);
+                        mma_tf32_8(s[nb], al1, bz, bw);
+                        mma_tf32_8(s[nb], ah1, to_tf32(x.z - bz), to_tf32(x.w - bw));
+                        mma_tf32_8(s[nb], ah1, bz, bw);
+                    }
+                }
+            } else {
+                const uint32_t kb = smem_u32(kt);
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k) {
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb += 2) {
+                        const int row = wk * KW + nb * 8 + ((lane >> 4) << 3) + (lane & 7);
+                        uint32_t b[4];
+                        ldsm4(b, kb + row * S::kRow + (((2 * k + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
+                        mma16<T>(s[nb], qf[k], b[0], b[1]);
+                        mma16<T>(s[nb + 1], qf[k], b[2], b[3]);
+                    }
+                }
+            }
+            // ---- running softmax in base 2
+            if (plain) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[nb][e] *= scale2;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int col = wk * KW + nb * 8 + 2 * cq + (e & 1);
+                        const int j = j0 + col, k = j - old;
+                        const int tok = e < 2 ? tok0 : tok1;
+                        bool see = tok >= 0 && j < rq.total && k_at[st][col] >= 0;
+                        if (see && k >= 0) {
+                            const uint32_t* mk = e < 2 ? mask0 : mask1;
+                            see = mk == nullptr ? k <= tok : (k >> 5) < g.mask_words && ((mk[k >> 5] >> (k & 31)) & 1u);
+                        }
+                        s[nb][e] = see ? s[nb][e] * scale2 : -INFINITY;
+                    }
+                }
+            }
+            float n0 = m0, n1 = m1;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                n0 = fmaxf(n0, fmaxf(s[nb][0], s[nb][1]));
+                n1 = fmaxf(n1, fmaxf(s[nb][2], s[nb][3]));
+            }
+            n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 1));
+            n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 2));
+            n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 1));
+            n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 2));
+            const float ref0 = n0 == -INFINITY ? 0.0f : n0, ref1 = n1 == -INFINITY ? 0.0f : n1;
+            const float keep0 = exp2_fast(m0 - ref0), keep1 = exp2_fast(m1 - ref1);
+            m0 = n0;
+            m1 = n1;
+            z0 *= keep0;
+            z1 *= keep1;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                s[nb][0] = exp2_fast(s[nb][0] - ref0);
+                s[nb][1] = exp2_fast(s[nb][1] - ref0);
+                s[nb][2] = exp2_fast(s[nb][2] - ref1);
+                s[nb][3] = exp2_fast(s[nb][3] - ref1);
+                z0 += s[nb][0] + s[nb][1];
+                z1 += s[nb][2] + s[nb][3];
+            }
+#pragma unroll
+            for (int i = 0; i < DP / 8; ++i) {
+                o[i][0] *= keep0;
+                o[i][1] *= keep0;
+                o[i][2] *= keep1;
+                o[i][3] *= keep1;
+            }
+            // ---- O += P V
+            if constexpr (S::kF32Type) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    // k index c and c + 4 are places 2c and 2c + 1: the layout the scores already have
+                    const float ph[4] = {to_tf32(s[nb][0]), to_tf32(s[nb][2]), to_tf32(s[nb][1]), to_tf32(s[nb][3])};
+                    const float pl[4] = {to_tf32(s[nb][0] - ph[0]), to_tf32(s[nb][2] - ph[1]),
+                                         to_tf32(s[nb][1] - ph[2]), to_tf32(s[nb][3] - ph[3])};
+                    const uint8_t* vr = vt + (wk * KW + nb * 8 + 2 * cq) * S::kRow + gq * 4;
+#pragma unroll
+                    for (int i = 0; i < DP / 8; ++i) {
+                        const float x = *reinterpret_cast<const float*>(vr + i * 32);
+                        const float y = *reinterpret_cast<const float*>(vr + S::kRow + i * 32);
+                        const float xh = to_tf32(x), yh = to_tf32(y);
+                        mma_tf32_8(o[i], pl, xh, yh);
+                        mma_tf32_8(o[i], ph, to_tf32(x - xh), to_tf32(y - yh));
+                        mma_tf32_8(o[i], ph, xh, yh);
+                    }
+                }
+            } else {
+                const uint32_t vb = smem_u32(vt);
+#pragma unroll
+                for (int nb = 0; nb < NB; nb += 2) {
+                    // weights to the cache's type: at most u off each, which the sum over places averages; the
+                    // sum z keeps all their bits
+                    const uint32_t p[4] = {pack2<T>(s[nb][0], s[nb][1]), pack2<T>(s[nb][2], s[nb][3]),
+                                           pack2<T>(s[nb + 1][0], s[nb + 1][1]), pack2<T>(s[nb + 1][2], s[nb + 1][3])};
+                    const int row = wk * KW + nb * 8 + (((lane >> 3) & 1) << 3) + (lane & 7);
+#pragma unroll
+                    for (int i = 0; i < DP / 16; ++i) {
+                        uint32_t b[4];
+                        ldsm4_t(b, vb + row * S::kRow + (((2 * i + (lane >> 4)) ^ (row & 7)) << 4));
+                        mma16<T>(o[2 * i], p, b[0], b[1]);
+                        mma16<T>(o[2 * i + 1], p, b[2], b[3]);
+                    }
+                }
+            }
+            if (!plain && odd_keys != 0) {
+                // values that are not finite, for the rows that see them
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        const int col = wk * KW + nb * 8 + c;
+                        if (((odd_keys >> col) & 1) == 0) {
+                            continue; // the same for the whole warp
+                        }
+                        const float p0 = __shfl_sync(0xffffffffu, s[nb][c & 1], (lane & 28) | (c >> 1));
+                        const float p1 = __shfl_sync(0xffffffffu, s[nb][2 + (c & 1)], (lane & 28) | (c >> 1));
+                        const T* v = static_cast<const T*>(a.vc) + v_at[st][col];
+#pragma unroll
+                        for (int i = 0; i < DP / 8; ++i) {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int d = i * 8 + 2 * cq + e;
+                                if (d < D) {
+                                    const float x = to_f32(v[d]);
+                                    o[i][e] += p0 > 0.0f ? p0 * x : 0.0f;
+                                    o[i][2 + e] += p1 > 0.0f ? p1 * x : 0.0f;
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+            place_rows(tile + NS - 1, next);
+            __syncthreads(); // every warp is done with the stage; the next tile's addresses are there
+            copy_tile(tile + NS - 1);
+        }
+        cp_wait<0>();
+        __syncthreads();
+
+        // ---- join the warps of each row group: sums over the ring's memory
+        z0 += __shfl_xor_sync(0xffffffffu, z0, 1);
+        z0 += __shfl_xor_sync(0xffffffffu, z0, 2);
+        z1 += __shfl_xor_sync(0xffffffffu, z1, 1);
+        z1 += __shfl_xor_sync(0xffffffffu, z1, 2);
+        float* join = reinterpret_cast<float*>(ring); // [WK][RT][DP]
+        {
+            const int l0 = wr * 16 + gq;
+            if (cq == 0) {
+                warp_ml[wk][l0] = make_float2(m0, z0);
+                warp_ml[wk][l0 + 8] = make_float2(m1, z1);
+            }
+            float* d0 = join + (wk * RT + l0) * DP + 2 * cq;
+#pragma unroll
+            for (int i = 0; i < DP / 8; ++i) {
+                *reinterpret_cast<float2*>(d0 + i * 8) = make_float2(o[i][0], o[i][1]);
+                *reinterpret_cast<float2*>(d0 + 8 * DP + i * 8) = make_float2(o[i][2], o[i][3]);
+            }
+        }
+        __syncthreads();
+        const bool whole = t_begin == 0 && t_end == rq.tiles;
+        const int my_slot = static_cast<int>(2 * cta) + (t_begin == 0 ? 1 : 0);
+        // four elements of a row a thread
+        auto store_row = [&](int row, int d, float4 x, float m, float z) {
+            const int rho = rb * RT + row, tok = rho / group;
+            const int64_t h = kvh * group + (rho - tok * group), t = rq.first + tok;
+            const bool none = z == 0.0f; // no place was seen
+            const float inv = 1.0f / z;
+            T* out = static_cast<T*>(a.out) + t * g.o_stride + h * g.o_head_stride + d;
+            Pack<T, 4> y;
+            y.e[0] = from_f32<T>(none ? 0.0f : x.x * inv);
+            y.e[1] = from_f32<T>(none ? 0.0f : x.y * inv);
+            y.e[2] = from_f32<T>(none ? 0.0f : x.z * inv);
+            y.e[3] = from_f32<T>(none ? 0.0f : x.w * inv);
+            *reinterpret_cast<Pack<T, 4>*>(out) = y;
+            if (d == 0 && a.lse != nullptr) {
+                a.lse[t * g.q_heads + h] = none ? -INFINITY : m * kLn2 + logf(z);
+            }
+        };
+        for (int i = tid; i < rows * (DP / 4); i += NT) {
+            const int row = i / (DP / 4), d = (i - row * (DP / 4)) * 4;
+            if (d >= D) {
                 continue;
             }
-            z += p[k];
-            const T* v = static_cast<const T*>(a.vc) + at[k];
-            if (tid < D) {
-                o0 += p[k] * to_f32(v[tid]);
+            float m = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < WK; ++k) {
+                m = fmaxf(m, warp_ml[k][row].x);
             }
-            if (tid + kSimpleThreads < D) {
-                o1 += p[k] * to_f32(v[tid + kSimpleThreads]);
+            const float ref = m == -INFINITY ? 0.0f : m;
+            float z = 0.0f;
+            float4 x = make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int k = 0; k < WK; ++k) {
+                const float2 ml = warp_ml[k][row];
+                const float f = exp2_fast(ml.x - ref);
+                const float4 y = *reinterpret_cast<const float4*>(join + (k * RT + row) * DP + d);
+                z += f * ml.y;
+                if (f != 0.0f) { // a part that saw nothing adds nothing
+                    x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
+                }
+            }
+            if (whole) {
+                store_row(row, d, x, m, z);
+            } else {
+                *reinterpret_cast<float4*>(part_o + (static_cast<int64_t>(my_slot) * RT + row) * DP + d) = x;
+                if (d == 0) {
+                    part_ml[static_cast<int64_t>(my_slot) * RT + row] = make_float2(m, z);
+                }
             }
         }
-        __syncthreads();
-    }
-    const float inv = z > 0.0f ? 1.0f / z : 0.0f;
-    if (tid < D) {
-        out[tid] = from_f32<T>(o0 * inv);
-    }
-    if (tid + kSimpleThreads < D) {
-        out[tid + kSimpleThreads] = from_f32<T>(o1 * inv);
-    }
-    if (tid == 0 && a.lse != nullptr) {
-        a.lse[t * g.q_heads + h] = z > 0.0f ? m + logf(z) : -INFINITY;
+        if (!whole) {
+            const int c0 = cta_of(item_w0, W, grid), c1 = cta_of(item_w1 - 1, W, grid);
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                const uint32_t n = atomicAdd(&tickets[c0], 1u);
+                is_last = n == static_cast<uint32_t>(c1 - c0);
+                if (is_last) {
+                    tickets[c0] = 0; // for the next launch
+                }
+            }
+            __syncthreads();
+            if (is_last) {
+                __threadfence();
+                for (int i = tid; i < rows * (DP / 4); i += NT) {
+                    const int row = i / (DP / 4), d = (i - row * (DP / 4)) * 4;
+                    if (d >= D) {
+                        continue;
+                    }
+                    float m = -INFINITY;
+                    for (int c = c0; c <= c1; ++c) {
+                        m = fmaxf(m, __ldcg(&part_ml[(2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0)) * RT + row]).x);
+                    }
+                    const float ref = m == -INFINITY ? 0.0f : m;
+                    float z = 0.0f;
+                    float4 x = make_float4(0, 0, 0, 0);
+                    for (int c = c0; c <= c1; ++c) {
+                        const int64_t slot = 2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0);
+                        const float2 ml = __ldcg(&part_ml[slot * RT + row]);
+                        const float f = exp2_fast(ml.x - ref);
+                        const float4 y = __ldcg(reinterpret_cast<const float4*>(part_o + (slot * RT + row) * DP + d));
+                        z += f * ml.y;
+                        if (f != 0.0f) {
+                            x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
+                        }
+                    }
+                    store_row(row, d, x, m, z);
+                }
+            }
+        }
+        w = item_w0 + t_end;
     }
     if (bad) {
         record_error(a.err, kDevIndexOutOfRange);
+    }
+}
+
+template <typename T, int DP, int WR, int WK>
+void launch_attn(nb2_device* dev, const TreeAttnArgs& a) {
+    using S = Shape<T, DP, WR, WK>;
+    auto kernel = tree_attn_kernel<T, DP, WR, WK>;
+    static int per_sm[64] = {};
+    if (per_sm[dev->ordinal] == 0) {
+        check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem),
+                   "cudaFuncSetAttribute(tree attention)");
+        int n = 0;
+        check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, S::kThreads, S::kSmem),
+                   "cudaOccupancyMaxActiveBlocksPerMultiprocessor");
+        per_sm[dev->ordinal] = std::max(1, n);
+    }
+    const int grid = dev->num_sms * per_sm[dev->ordinal];
+    const size_t o_bytes = static_cast<size_t>(grid) * 2 * S::RT * DP * 4;
+    uint8_t* ws = static_cast<uint8_t*>(dev->scratch(o_bytes + static_cast<size_t>(grid) * 2 * S::RT * 8));
+    kernel<<<grid, S::kThreads, S::kSmem, dev->stream>>>(a, static_cast<int>(a.g.q_heads / a.g.kv_heads),
+                                                         reinterpret_cast<float*>(ws),
+                                                         reinterpret_cast<float2*>(ws + o_bytes), dev->tickets(grid));
+    check_cuda(cudaGetLastError(), "tree attention launch");
+}
+
+template <typename T, int DP>
+void pick_rows(nb2_device* dev, const TreeAttnArgs& a) {
+    const int64_t rows = std::min(a.g.max_new, a.g.tokens) * (a.g.q_heads / a.g.kv_heads);
+    if (rows <= 16) {
+        launch_attn<T, DP, 1, 4>(dev, a);
+    } else if (rows <= 32 || DP * sizeof(T) > 512) { // 64 rows of 256 float32 in two parts do not fit
+        launch_attn<T, DP, 2, 4>(dev, a);
+    } else if constexpr (DP * sizeof(T) <= 512) {
+        launch_attn<T, DP, 4, 2>(dev, a);
+    }
+}
+
+template <typename T>
+void pick_dim(nb2_device* dev, const TreeAttnArgs& a) {
+    if (a.g.head_dim <= 64) {
+        pick_rows<T, 64>(dev, a);
+    } else if (a.g.head_dim <= 128) {
+        pick_rows<T, 128>(dev, a);
+    } else {
+        pick_rows<T, 256>(dev, a);
     }
 }
 
@@ -132,15 +787,13 @@ void tree_attention(nb2_device* dev, TreeAttnArgs a) {
         return;
     }
     a.err = dev->err_word;
-    const dim3 grid(static_cast<unsigned>(a.g.tokens), static_cast<unsigned>(a.g.q_heads));
     if (a.g.dtype == kF32) {
-        tree_attn_kernel<float><<<grid, kSimpleThreads, 0, dev->stream>>>(a);
+        pick_dim<float>(dev, a);
     } else if (a.g.dtype == kF16) {
-        tree_attn_kernel<__half><<<grid, kSimpleThreads, 0, dev->stream>>>(a);
+        pick_dim<__half>(dev, a);
     } else {
-        tree_attn_kernel<__nv_bfloat16><<<grid, kSimpleThreads, 0, dev->stream>>>(a);
+        pick_dim<__nv_bfloat16>(dev, a);
     }
-    check_cuda(cudaGetLastError(), "tree attention launch");
 }
 
 } // namespace nb2

@@ -358,6 +358,29 @@ def test_tree_attention_rows_that_see_nothing(cuda, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("news,g", [([9, 40], 1), ([70, 40], 4)])
+def test_tree_attention_masked_places_that_are_not_finite(cuda, dtype, news, g):
+    """A drafted token whose key and value are infinite or NaN reaches the tokens that see it and no others."""
+    b = Batch([50, 300], news, 2 * g, 2, 128, 16, dtype, trees="star")  # each drafted token sees itself only
+    for r, i, val in ((0, 2, float("inf")), (1, 7, float("nan")), (1, 30, -float("inf"))):
+        p = int(b.old[r]) + i
+        block = int(b.table[r, p // 16])
+        b.vc[block, p % 16] = val
+        if val != val:
+            b.kc[block, p % 16] = val
+    out, lse = b.run()
+    serving.synchronize()
+    hit = [int(b.off[0]) + 2, int(b.off[1]) + 7, int(b.off[1]) + 30]
+    assert not torch.isfinite(out[hit]).any()
+    assert torch.isnan(lse[hit[1]]).all() and torch.isfinite(lse[hit[0]]).all()
+    rest = [t for t in range(out.shape[0]) if t not in hit]
+    clean = Batch([50, 300], news, 2 * g, 2, 128, 16, dtype, trees="star")
+    want, want_lse = clean.run()
+    serving.synchronize()
+    assert torch.equal(out[rest], want[rest]) and torch.equal(lse[rest], want_lse[rest])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_tree_attention_large_scores(cuda, dtype):
     """Scores of several hundred: the running maximum moves, and weights underflow."""
     b = Batch([500, 130], [9, 40], 4, 1, 128, 16, dtype, spread=40.0)
