@@ -7,6 +7,9 @@
   (``device/b200_device.cpp``), compiled against the NERT public headers when
   they are available (``NERT_INCLUDE``, else the ``include/`` of the reference
   checkout named by ``NERT_REFERENCE`` or lying beside this repository).
+* ``nert_b200/lib/nert_b200_torch.so`` — the Python module behind
+  ``nert_b200.serving`` (``csrc/torch/serving_torch.cpp``), compiled against
+  the installed torch's headers.
 
 Objects are rebuilt only when a source or header is newer than the object.
 """
@@ -32,6 +35,7 @@ CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall"]
 
 MAIN_LIB = os.path.join(LIB_DIR, "libnert_b200.so")
 DEVICE_LIB = os.path.join(LIB_DIR, "libnert_b200_device.so")
+TORCH_LIB = os.path.join(LIB_DIR, "nert_b200_torch.so")
 
 
 def nert_include() -> str | None:
@@ -105,9 +109,36 @@ def build_device_plugin(verbose: bool = False) -> str | None:
     return DEVICE_LIB
 
 
+def build_torch_module(verbose: bool = False) -> str:
+    """The Python module of the serving rows, against the installed torch."""
+    src = os.path.join(HERE, "csrc", "torch", "serving_torch.cpp")
+    hdr = os.path.join(ROOT, "include", "nert_b200.h")
+    if os.path.exists(TORCH_LIB) and os.path.getmtime(TORCH_LIB) >= _newest([src, hdr]):
+        return TORCH_LIB
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    inc = [f"-I{p}" for p in (*cpp_extension.include_paths(), os.path.join(CUDA_HOME, "include"),
+                              sysconfig.get_paths()["include"])]
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = ["g++", *CXX_FLAGS, "-Wno-deprecated-declarations", "-shared", "-DTORCH_EXTENSION_NAME=nert_b200_torch",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc, src, "-o", TORCH_LIB,
+           f"-L{libs}", "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10_cuda", f"-Wl,-rpath,{libs}",
+           "-L", LIB_DIR, "-lnert_b200", "-Wl,-rpath,$ORIGIN"]
+    out = subprocess.run(cmd, capture_output=True, text=True)
+    if out.returncode != 0:
+        raise RuntimeError(f"torch module build failed: {' '.join(cmd)}\n{out.stdout}\n{out.stderr}")
+    if verbose:
+        print("built", os.path.relpath(TORCH_LIB, ROOT))
+    return TORCH_LIB
+
+
 def build(verbose: bool = False) -> None:
     os.makedirs(LIB_DIR, exist_ok=True)
     build_main(verbose)
+    build_torch_module(verbose)
     build_device_plugin(verbose)
 
 

@@ -465,12 +465,19 @@ __global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(TreeAttnArgs a,
                         const float4 x = *reinterpret_cast<const float4*>(kt + (wk * KW + nb * 8 + gq) * S::kRow +
                                                                           (4 * k + cq) * 16);
                         const float bx = to_tf32(x.x), by = to_tf32(x.y), bz = to_tf32(x.z), bw = to_tf32(x.w);
-                        mma_tf32_8(s[nb], al0, bx, by);
-                        mma_tf32_8(s[nb], ah0, to_tf32(x.x - bx), to_tf32(x.y - by));
-                        mma_tf32_8(s[nb], ah0, bx, by);
-                        mma_tf32_8(s[nb], al1, bz, bw);
-                        mma_tf32_8(s[nb], ah1, to_tf32(x.z - bz), to_tf32(x.w - bw));
-                        mma_tf32_8(s[nb], ah1, bz, bw);
+                        // the tensor cores truncate where they add: chains are kept short and summed
+                        // in round-to-nearest (one long chain measured twice the error)
+                        float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        mma_tf32_8(t, al0, bx, by);
+                        mma_tf32_8(t, ah0, to_tf32(x.x - bx), to_tf32(x.y - by));
+                        mma_tf32_8(t, al1, bz, bw);
+                        mma_tf32_8(t, ah1, to_tf32(x.z - bz), to_tf32(x.w - bw));
+                        mma_tf32_8(t, ah0, bx, by);
+                        mma_tf32_8(t, ah1, bz, bw);
+                        s[nb][0] += t[0];
+                        s[nb][1] += t[1];
+                        s[nb][2] += t[2];
+                        s[nb][3] += t[3];
                     }
                 }
             } else {
@@ -538,31 +545,45 @@ __global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(TreeAttnArgs a,
                 z0 += s[nb][0] + s[nb][1];
                 z1 += s[nb][2] + s[nb][3];
             }
+            if constexpr (!S::kF32Type) {
 #pragma unroll
-            for (int i = 0; i < DP / 8; ++i) {
-                o[i][0] *= keep0;
-                o[i][1] *= keep0;
-                o[i][2] *= keep1;
-                o[i][3] *= keep1;
+                for (int i = 0; i < DP / 8; ++i) {
+                    o[i][0] *= keep0;
+                    o[i][1] *= keep0;
+                    o[i][2] *= keep1;
+                    o[i][3] *= keep1;
+                }
             }
             // ---- O += P V
             if constexpr (S::kF32Type) {
+                float ph[NB][4], pl[NB][4];
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
                     // k index c and c + 4 are places 2c and 2c + 1: the layout the scores already have
-                    const float ph[4] = {to_tf32(s[nb][0]), to_tf32(s[nb][2]), to_tf32(s[nb][1]), to_tf32(s[nb][3])};
-                    const float pl[4] = {to_tf32(s[nb][0] - ph[0]), to_tf32(s[nb][2] - ph[1]),
-                                         to_tf32(s[nb][1] - ph[2]), to_tf32(s[nb][3] - ph[3])};
-                    const uint8_t* vr = vt + (wk * KW + nb * 8 + 2 * cq) * S::kRow + gq * 4;
+                    const float p[4] = {s[nb][0], s[nb][2], s[nb][1], s[nb][3]};
 #pragma unroll
-                    for (int i = 0; i < DP / 8; ++i) {
-                        const float x = *reinterpret_cast<const float*>(vr + i * 32);
-                        const float y = *reinterpret_cast<const float*>(vr + S::kRow + i * 32);
-                        const float xh = to_tf32(x), yh = to_tf32(y);
-                        mma_tf32_8(o[i], pl, xh, yh);
-                        mma_tf32_8(o[i], ph, to_tf32(x - xh), to_tf32(y - yh));
-                        mma_tf32_8(o[i], ph, xh, yh);
+                    for (int e = 0; e < 4; ++e) {
+                        ph[nb][e] = to_tf32(p[e]);
+                        pl[nb][e] = to_tf32(p[e] - ph[nb][e]);
                     }
+                }
+                const uint8_t* vr = vt + (wk * KW + 2 * cq) * S::kRow + gq * 4;
+#pragma unroll
+                for (int i = 0; i < DP / 8; ++i) {
+                    float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        const float x = *reinterpret_cast<const float*>(vr + nb * 8 * S::kRow + i * 32);
+                        const float y = *reinterpret_cast<const float*>(vr + (nb * 8 + 1) * S::kRow + i * 32);
+                        const float xh = to_tf32(x), yh = to_tf32(y);
+                        mma_tf32_8(t, pl[nb], xh, yh);
+                        mma_tf32_8(t, ph[nb], to_tf32(x - xh), to_tf32(y - yh));
+                        mma_tf32_8(t, ph[nb], xh, yh);
+                    }
+                    o[i][0] = fmaf(o[i][0], keep0, t[0]);
+                    o[i][1] = fmaf(o[i][1], keep0, t[1]);
+                    o[i][2] = fmaf(o[i][2], keep1, t[2]);
+                    o[i][3] = fmaf(o[i][3], keep1, t[3]);
                 }
             } else {
                 const uint32_t vb = smem_u32(vt);
