@@ -175,7 +175,10 @@ int nb2_logits_process(nb2_device* dev, const nb2_logits_geom* g, const void* lo
              "LogitsProcess: a list needs its offsets");
         need(bias_ids == nullptr || (bias_values != nullptr && bias_offsets != nullptr),
              "LogitsProcess: a bias list needs its values and offsets");
-        need(in_i32(g->prompt_count) && in_i32(g->output_count) && in_i32(g->bias_count), "LogitsProcess: bad list sizes");
+        constexpr int64_t kMaxList = int64_t{1} << 30; // a count of one token must fit 30 bits
+        need(g->prompt_count >= 0 && g->prompt_count < kMaxList && g->output_count >= 0 &&
+                 g->output_count < kMaxList && g->bias_count >= 0 && g->bias_count < kMaxList,
+             "LogitsProcess: a list holds between 0 and 2^30 - 1 ids");
         need(grammar == nullptr || g->grammar_stride >= (g->vocab + 31) / 32, "LogitsProcess: a grammar row is too short");
         if (g->rows == 0 || g->vocab == 0) {
             return;
