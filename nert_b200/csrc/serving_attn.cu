@@ -23,74 +23,13 @@
 // through a ring of NS stages, the addresses of a tile's rows looked up in the block table one tile
 // ahead of its copies.
 
-#include "serving.cuh"
+#include "serving_attn.cuh"
 
 #include <type_traits>
 
 namespace nb2 {
 
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-
-// ---- the split of the work ----------------------------------------------------
-
-struct Request {
-    int64_t first;  // its first token
-    int n, total;   // new tokens, places (0 where the lengths cannot be right)
-    int row_blocks; // blocks of its n * group rows
-    int tiles;      // tiles of its places, at least one so that rows without places are written
-    bool bad;
-    __device__ __forceinline__ int64_t units(int64_t kv_heads) const {
-        return static_cast<int64_t>(row_blocks) * kv_heads * tiles;
-    }
-};
-
-template <int RT, int KT>
-__device__ __forceinline__ Request request_at(const TreeAttnArgs& a, int r, int group) {
-    Request q{};
-    const int64_t lo = a.offsets[r], hi = a.offsets[r + 1];
-    const int64_t total = a.total[r];
-    if (lo < 0 || hi < lo || hi > a.g.tokens) {
-        q.bad = true;
-        return q;
-    }
-    q.first = lo;
-    q.n = static_cast<int>(hi - lo);
-    if (q.n == 0) {
-        return q;
-    }
-    q.bad = total < q.n || total > a.g.table_blocks * a.g.block_size || q.n > a.g.max_new;
-    q.total = q.bad ? 0 : static_cast<int>(total);
-    q.row_blocks = static_cast<int>((static_cast<int64_t>(q.n) * group + RT - 1) / RT);
-    q.tiles = max(1, (q.total + KT - 1) / KT);
-    return q;
-}
-
-// CTA whose span holds unit w, of `grid` spans [c W / grid, (c + 1) W / grid).
-__device__ __forceinline__ int cta_of(int64_t w, int64_t W, int64_t grid) {
-    return static_cast<int>(((w + 1) * grid - 1) / W);
-}
-
-template <int NT>
-__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* red) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        v += __shfl_xor_sync(0xffffffffu, v, o);
-    }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) {
-        red[threadIdx.x >> 5] = v;
-    }
-    __syncthreads();
-    int64_t s = 0;
-#pragma unroll
-    for (int w = 0; w < NT / 32; ++w) {
-        s += red[w];
-    }
-    return s;
-}
 
 // ---- instructions ----------------------------------------------------------------
 
@@ -149,12 +88,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     }
 }
 
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // ---- the kernel -----------------------------------------------------------------
 
 template <typename T, int DP, int WR, int WK>
@@ -189,88 +122,28 @@ __global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(TreeAttnArgs a,
     __shared__ int holes[NS][KT / 32];             // a place inside total has no block
     __shared__ unsigned long long odd_keys;        // places of the tile whose values are not finite
     __shared__ float2 warp_ml[WK][RT];
-    __shared__ int64_t start_unit;
-    __shared__ int start_request, is_last;
+    __shared__ int64_t found[2];
+    __shared__ int is_last;
 
     const nb2_tree_attn_geom& g = a.g;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int wr = warp / WK, wk = warp % WK;
     const int gq = lane >> 2, cq = lane & 3;
-    const int B = static_cast<int>(g.batch);
     const int64_t cta = blockIdx.x;
     const int D = static_cast<int>(g.head_dim);
     const float scale2 = g.scale * kLog2e;
     bool bad = false;
 
-    // ---- this CTA's span
-    int64_t sum = 0;
-    for (int r = tid; r < B; r += NT) {
-        const Request q = request_at<RT, KT>(a, r, group);
-        bad |= q.bad;
-        sum += q.units(g.kv_heads);
-    }
-    const int64_t W = block_sum<NT>(sum, red);
-    // tokens that belong to no request
-    {
-        const int64_t lo = B > 0 ? a.offsets[0] : 0, hi = B > 0 ? a.offsets[B] : 0;
-        const int64_t before = min(max(lo, int64_t{0}), g.tokens), after = min(max(hi, before), g.tokens);
-        const int64_t spare = (before + g.tokens - after) * g.q_heads;
-        for (int64_t i = cta * NT + tid; i < spare; i += static_cast<int64_t>(gridDim.x) * NT) {
-            int64_t t = i / g.q_heads;
-            const int64_t h = i - t * g.q_heads;
-            t = t < before ? t : t - before + after;
-            T* row = static_cast<T*>(a.out) + t * g.o_stride + h * g.o_head_stride;
-            for (int d = 0; d < D; ++d) {
-                row[d] = from_f32<T>(0.0f);
-            }
-            if (a.lse != nullptr) {
-                a.lse[t * g.q_heads + h] = -INFINITY;
-            }
-        }
-    }
-    const int64_t grid = min(static_cast<int64_t>(gridDim.x), W); // no span is empty
-    const int64_t w0 = cta < grid ? cta * W / grid : 0, w1 = cta < grid ? (cta + 1) * W / grid : 0;
-    if (w0 < w1) {
-        int64_t base = 0;
-        for (int c = 0; c < B; c += NT) { // the request that holds unit w0
-            const int64_t u = c + tid < B ? request_at<RT, KT>(a, c + tid, group).units(g.kv_heads) : 0;
-            int64_t inc = u;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t up = __shfl_up_sync(0xffffffffu, inc, o);
-                inc += lane >= o ? up : 0;
-            }
-            __syncthreads();
-            if (lane == 31) {
-                red[warp] = inc;
-            }
-            __syncthreads();
-            int64_t all = 0;
-#pragma unroll
-            for (int w = 0; w < NT / 32; ++w) {
-                inc += w < warp ? red[w] : 0;
-                all += red[w];
-            }
-            inc += base;
-            if (inc - u <= w0 && w0 < inc) {
-                start_request = c + tid;
-                start_unit = inc - u;
-            }
-            base += all;
-            if (base > w0) {
-                break;
-            }
-        }
-        __syncthreads();
-    }
-
-    int r = w0 < w1 ? start_request : 0;
-    int64_t r_unit = w0 < w1 ? start_unit : 0; // first unit of request r
+    const Span span = find_span<RT, KT, NT>(a, group, red, found, bad);
+    spare_tokens<T>(a, tid, NT);
+    const int64_t W = span.W, grid = span.grid, w1 = span.w1;
+    int r = span.request;
+    int64_t r_unit = span.request_unit; // first unit of request r
     Request rq{};
-    if (w0 < w1) {
+    if (span.w0 < w1) {
         rq = request_at<RT, KT>(a, r, group);
     }
-    for (int64_t w = w0; w < w1;) {
+    for (int64_t w = span.w0; w < w1;) {
         while (w >= r_unit + rq.units(g.kv_heads)) {
             r_unit += rq.units(g.kv_heads);
             rq = request_at<RT, KT>(a, ++r, group);
@@ -660,23 +533,6 @@ __global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(TreeAttnArgs a,
         __syncthreads();
         const bool whole = t_begin == 0 && t_end == rq.tiles;
         const int my_slot = static_cast<int>(2 * cta) + (t_begin == 0 ? 1 : 0);
-        // four elements of a row a thread
-        auto store_row = [&](int row, int d, float4 x, float m, float z) {
-            const int rho = rb * RT + row, tok = rho / group;
-            const int64_t h = kvh * group + (rho - tok * group), t = rq.first + tok;
-            const bool none = z == 0.0f; // no place was seen
-            const float inv = 1.0f / z;
-            T* out = static_cast<T*>(a.out) + t * g.o_stride + h * g.o_head_stride + d;
-            Pack<T, 4> y;
-            y.e[0] = from_f32<T>(none ? 0.0f : x.x * inv);
-            y.e[1] = from_f32<T>(none ? 0.0f : x.y * inv);
-            y.e[2] = from_f32<T>(none ? 0.0f : x.z * inv);
-            y.e[3] = from_f32<T>(none ? 0.0f : x.w * inv);
-            *reinterpret_cast<Pack<T, 4>*>(out) = y;
-            if (d == 0 && a.lse != nullptr) {
-                a.lse[t * g.q_heads + h] = none ? -INFINITY : m * kLn2 + logf(z);
-            }
-        };
         for (int i = tid; i < rows * (DP / 4); i += NT) {
             const int row = i / (DP / 4), d = (i - row * (DP / 4)) * 4;
             if (d >= D) {
@@ -701,7 +557,7 @@ __global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(TreeAttnArgs a,
                 }
             }
             if (whole) {
-                store_row(row, d, x, m, z);
+                store_row4<T>(a, rq.first, kvh, group, rb * RT + row, d, x, m, z);
             } else {
                 *reinterpret_cast<float4*>(part_o + (static_cast<int64_t>(my_slot) * RT + row) * DP + d) = x;
                 if (d == 0) {
@@ -723,30 +579,7 @@ __global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(TreeAttnArgs a,
             __syncthreads();
             if (is_last) {
                 __threadfence();
-                for (int i = tid; i < rows * (DP / 4); i += NT) {
-                    const int row = i / (DP / 4), d = (i - row * (DP / 4)) * 4;
-                    if (d >= D) {
-                        continue;
-                    }
-                    float m = -INFINITY;
-                    for (int c = c0; c <= c1; ++c) {
-                        m = fmaxf(m, __ldcg(&part_ml[(2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0)) * RT + row]).x);
-                    }
-                    const float ref = m == -INFINITY ? 0.0f : m;
-                    float z = 0.0f;
-                    float4 x = make_float4(0, 0, 0, 0);
-                    for (int c = c0; c <= c1; ++c) {
-                        const int64_t slot = 2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0);
-                        const float2 ml = __ldcg(&part_ml[slot * RT + row]);
-                        const float f = exp2_fast(ml.x - ref);
-                        const float4 y = __ldcg(reinterpret_cast<const float4*>(part_o + (slot * RT + row) * DP + d));
-                        z += f * ml.y;
-                        if (f != 0.0f) {
-                            x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
-                        }
-                    }
-                    store_row(row, d, x, m, z);
-                }
+                join_pieces<T, DP, RT, NT>(a, part_o, part_ml, c0, c1, rq.first, kvh, group, rb * RT, rows, tid);
             }
         }
         w = item_w0 + t_end;
@@ -808,7 +641,9 @@ void tree_attention(nb2_device* dev, TreeAttnArgs a) {
         return;
     }
     a.err = dev->err_word;
-    if (a.g.dtype == kF32) {
+    if (tree_attention_tc_takes(a)) {
+        tree_attention_tc(dev, a);
+    } else if (a.g.dtype == kF32) {
         pick_dim<float>(dev, a);
     } else if (a.g.dtype == kF16) {
         pick_dim<__half>(dev, a);

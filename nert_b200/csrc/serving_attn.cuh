@@ -1,0 +1,215 @@
+// Shared by the tree attention kernels: the split of the work over the grid and
+// the join of the pieces. The split is explained in serving_attn.cu.
+#pragma once
+
+#include "serving.cuh"
+
+namespace nb2 {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// ---- the split of the work ----------------------------------------------------
+
+struct Request {
+    int64_t first;  // its first token
+    int n, total;   // new tokens, places (0 where the lengths cannot be right)
+    int row_blocks; // blocks of its n * group rows
+    int tiles;      // tiles of its places, at least one so that rows without places are written
+    bool bad;
+    __device__ __forceinline__ int64_t units(int64_t kv_heads) const {
+        return static_cast<int64_t>(row_blocks) * kv_heads * tiles;
+    }
+};
+
+template <int RT, int KT>
+__device__ __forceinline__ Request request_at(const TreeAttnArgs& a, int r, int group) {
+    Request q{};
+    const int64_t lo = a.offsets[r], hi = a.offsets[r + 1];
+    const int64_t total = a.total[r];
+    if (lo < 0 || hi < lo || hi > a.g.tokens) {
+        q.bad = true;
+        return q;
+    }
+    q.first = lo;
+    q.n = static_cast<int>(hi - lo);
+    if (q.n == 0) {
+        return q;
+    }
+    q.bad = total < q.n || total > a.g.table_blocks * a.g.block_size || q.n > a.g.max_new;
+    q.total = q.bad ? 0 : static_cast<int>(total);
+    q.row_blocks = static_cast<int>((static_cast<int64_t>(q.n) * group + RT - 1) / RT);
+    q.tiles = max(1, (q.total + KT - 1) / KT);
+    return q;
+}
+
+// CTA whose span holds unit w, of `grid` spans [c W / grid, (c + 1) W / grid).
+__device__ __forceinline__ int cta_of(int64_t w, int64_t W, int64_t grid) {
+    return static_cast<int>(((w + 1) * grid - 1) / W);
+}
+
+template <int NT>
+__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* red) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+    }
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) {
+        red[threadIdx.x >> 5] = v;
+    }
+    __syncthreads();
+    int64_t s = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) {
+        s += red[w];
+    }
+    return s;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// ---- the join ------------------------------------------------------------------
+
+// Elements d .. d + 3 of a finished row (unnormalised sums x, maximum m in base 2, sum of weights z).
+template <typename T>
+__device__ __forceinline__ void store_row4(const TreeAttnArgs& a, int64_t first, int64_t kvh, int group, int rho, int d,
+                                           float4 x, float m, float z) {
+    const int tok = rho / group;
+    const int64_t h = kvh * group + (rho - tok * group), t = first + tok;
+    const bool none = z == 0.0f; // no place was seen
+    const float inv = 1.0f / z;
+    Pack<T, 4> y;
+    y.e[0] = from_f32<T>(none ? 0.0f : x.x * inv);
+    y.e[1] = from_f32<T>(none ? 0.0f : x.y * inv);
+    y.e[2] = from_f32<T>(none ? 0.0f : x.z * inv);
+    y.e[3] = from_f32<T>(none ? 0.0f : x.w * inv);
+    *reinterpret_cast<Pack<T, 4>*>(static_cast<T*>(a.out) + t * a.g.o_stride + h * a.g.o_head_stride + d) = y;
+    if (d == 0 && a.lse != nullptr) {
+        a.lse[t * a.g.q_heads + h] = none ? -INFINITY : m * kLn2 + logf(z);
+    }
+}
+
+// The pieces of an item in the slots of CTAs c0 .. c1 (the first left its piece in its second slot,
+// the others theirs in their first), added in that order and stored; NT threads.
+template <typename T, int DP, int RT, int NT>
+__device__ __forceinline__ void join_pieces(const TreeAttnArgs& a, const float* part_o, const float2* part_ml, int c0, int c1,
+                                            int64_t first, int64_t kvh, int group, int rho0, int rows, int tid) {
+    for (int i = tid; i < rows * (DP / 4); i += NT) {
+        const int row = i / (DP / 4), d = (i - row * (DP / 4)) * 4;
+        if (d >= a.g.head_dim) {
+            continue;
+        }
+        float m = -INFINITY;
+        for (int c = c0; c <= c1; ++c) {
+            m = fmaxf(m, __ldcg(&part_ml[(2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0)) * RT + row]).x);
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+        float z = 0.0f;
+        float4 x = make_float4(0, 0, 0, 0);
+        for (int c = c0; c <= c1; ++c) {
+            const int64_t slot = 2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0);
+            const float2 ml = __ldcg(&part_ml[slot * RT + row]);
+            const float f = exp2_fast(ml.x - ref);
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(part_o + (slot * RT + row) * DP + d));
+            z += f * ml.y;
+            if (f != 0.0f) { // a piece that saw nothing adds nothing
+                x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
+            }
+        }
+        store_row4<T>(a, first, kvh, group, rho0 + row, d, x, m, z);
+    }
+}
+
+// Zero rows for the tokens that belong to no request.
+template <typename T>
+__device__ __forceinline__ void spare_tokens(const TreeAttnArgs& a, int tid, int nt) {
+    const nb2_tree_attn_geom& g = a.g;
+    const int64_t lo = g.batch > 0 ? a.offsets[0] : 0, hi = g.batch > 0 ? a.offsets[g.batch] : 0;
+    const int64_t before = min(max(lo, int64_t{0}), g.tokens), after = min(max(hi, before), g.tokens);
+    const int64_t spare = (before + g.tokens - after) * g.q_heads;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * nt + tid; i < spare; i += static_cast<int64_t>(gridDim.x) * nt) {
+        int64_t t = i / g.q_heads;
+        const int64_t h = i - t * g.q_heads;
+        t = t < before ? t : t - before + after;
+        T* row = static_cast<T*>(a.out) + t * g.o_stride + h * g.o_head_stride;
+        for (int d = 0; d < g.head_dim; ++d) {
+            row[d] = from_f32<T>(0.0f);
+        }
+        if (a.lse != nullptr) {
+            a.lse[t * g.q_heads + h] = -INFINITY;
+        }
+    }
+}
+
+// This CTA's span of the W units, and the request that its first unit is in. All NT threads.
+struct Span {
+    int64_t W, grid, w0, w1;
+    int request;          // holds unit w0
+    int64_t request_unit; // first unit of that request
+};
+
+template <int RT, int KT, int NT>
+__device__ __forceinline__ Span find_span(const TreeAttnArgs& a, int group, int64_t* red, int64_t* found, bool& bad) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int B = static_cast<int>(a.g.batch);
+    const int64_t cta = blockIdx.x;
+    Span s{};
+    int64_t sum = 0;
+    for (int r = tid; r < B; r += NT) {
+        const Request q = request_at<RT, KT>(a, r, group);
+        bad |= q.bad;
+        sum += q.units(a.g.kv_heads);
+    }
+    s.W = block_sum<NT>(sum, red);
+    s.grid = min(static_cast<int64_t>(gridDim.x), s.W); // no span is empty
+    if (cta >= s.grid) {
+        return s;
+    }
+    s.w0 = cta * s.W / s.grid;
+    s.w1 = (cta + 1) * s.W / s.grid;
+    int64_t base = 0;
+    for (int c = 0; c < B; c += NT) {
+        const int64_t u = c + tid < B ? request_at<RT, KT>(a, c + tid, group).units(a.g.kv_heads) : 0;
+        int64_t inc = u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t up = __shfl_up_sync(0xffffffffu, inc, o);
+            inc += lane >= o ? up : 0;
+        }
+        __syncthreads();
+        if (lane == 31) {
+            red[warp] = inc;
+        }
+        __syncthreads();
+        int64_t all = 0;
+#pragma unroll
+        for (int w = 0; w < NT / 32; ++w) {
+            inc += w < warp ? red[w] : 0;
+            all += red[w];
+        }
+        inc += base;
+        if (inc - u <= s.w0 && s.w0 < inc) {
+            found[0] = c + tid;
+            found[1] = inc - u;
+        }
+        base += all;
+        if (base > s.w0) {
+            break;
+        }
+    }
+    __syncthreads();
+    s.request = static_cast<int>(found[0]);
+    s.request_unit = found[1];
+    return s;
+}
+
+// The tensor-core kernel for many rows (serving_attn_tc.cu): whether it takes the call, and the call.
+bool tree_attention_tc_takes(const TreeAttnArgs& a);
+void tree_attention_tc(nb2_device* dev, const TreeAttnArgs& a);
+
+} // namespace nb2

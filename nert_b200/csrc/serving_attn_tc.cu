@@ -1,0 +1,817 @@
+// Tree attention for many rows a key/value head (wide trees, large groups), on
+// the tcgen05 tensor cores: 16-bit types, head dimensions 64 to 128, pages of a
+// power of two. The split of the work, the masks and the join are those of
+// serving_attn.cu; with 33 rows and more that kernel is bound by its mma.sync and
+// shared-memory rate, this one by exponentials (16 a clock and SM) or by HBM.
+//
+// One CTA an SM, ten warps: two softmax groups of four warps, a TMA warp, an MMA thread. K and V
+// tiles of 128 places come page by page as 4-D TMA boxes (64 elements x page) into 128-byte
+// swizzled slabs, through rings of their own. Tensor memory holds two score tiles S (128 rows x 128
+// places, fp32) and two accumulators O; group s owns S and O number s, one row a thread, so a row's
+// maximum and sum need no exchange between threads. It reads S, writes the weights P as packed 16-bit over
+// S's first half, and the MMA thread multiplies P from there with V (whose keys are the contraction:
+// V is the MN-major operand as it lies in the cache).
+//   kTiles = 2: the groups are two blocks of 128 rows and share every tile of places.
+//   kTiles = 1: up to 128 rows; the groups take alternate tiles of the same rows, and join at the end.
+// So one group's softmax runs while the other's products do. O is rescaled in place, by its own
+// group, only when a row's maximum has grown by more than 2^8 since its reference was set (the
+// weights and sums stay far inside the range of their types; the final division takes the reference out).
+//
+// Values that are not finite, and rows past the end of a page list, would reach rows that do not see them
+// as 0 * inf: in the tiles that hold new tokens (or holes) the group clears such rows of V in shared
+// memory before its P is released, and adds p * v itself for the rows that see the place.
+//
+// Every wait is bounded; a thread that gives up raises the CTA's abort flag, after which all loops run
+// out without waiting, touching tensor memory or storing results.
+
+#include "serving_attn.cuh"
+
+#include <type_traits>
+
+namespace nb2 {
+
+namespace {
+
+constexpr int kTcThreads = 320;
+constexpr int kSoftmax = 256; // threads of the two softmax groups
+constexpr int kTile = 128;    // places of a tile, rows of a block
+constexpr uint32_t kColO = 256;
+constexpr int kTcRows = 32; // rows a key/value head above which this kernel is taken
+
+// ---- instructions -------------------------------------------------------------
+
+// Shared-memory matrix descriptor, 128-byte swizzle (see sdesc_k128), with its leading byte offset: for an MN-major
+// operand the distance of the next 64 elements of N.
+__device__ __forceinline__ uint64_t sdesc_128(uint32_t saddr, uint32_t lbo) {
+    return static_cast<uint64_t>((saddr & 0x3FFFF) >> 4) | (static_cast<uint64_t>(lbo >> 4) << 16) | (64ull << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+
+// kind::f16, fp32 accumulator, M = 128: operand type, N, and whether B is MN-major.
+__host__ __device__ constexpr uint32_t idesc_f16(bool bf16, int n, bool b_mn) {
+    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) |
+           (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
+}
+
+// D[tmem] (+)= A[smem] * B[smem]
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+
+// D[tmem] += A[tmem] * B[smem]; A is 16-bit, two elements a column
+__device__ __forceinline__ void mma_f16_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+                 "r"(a), "l"(b), "r"(idesc), "r"(1u)
+                 : "memory");
+}
+
+// 32 lanes x 32 columns to registers; complete with tmem_wait_ld().
+__device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+                 "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+                   "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+                   "=r"(r[30]), "=r"(r[31])
+                 : "r"(t));
+}
+__device__ __forceinline__ void tmem_ld1(uint32_t t, uint32_t& r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(t));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_st32(uint32_t t, const uint32_t (&r)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+                 "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(t),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+                 "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+                 "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+                 "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+                 : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16u(uint32_t t, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+                     t),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+                 "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+
+// A page's 64 elements x box rows; coordinates element, head, place, block (out of range reads zeros). No multicast.
+__device__ __forceinline__ void tma_load_page(void* dst, const CUtensorMap* map, int e, int head, int place, int block,
+                                              uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+                 " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(e), "r"(head), "r"(place), "r"(block)
+                 : "memory");
+}
+
+__device__ __forceinline__ void bar_named(int id, int threads) {
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (std::is_same_v<T, __half>) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+
+// Bits of places k0 .. k0 + 31, counted from the first new token, that a row's token sees.
+__device__ __forceinline__ uint32_t see_bits(const uint32_t* mask, int64_t words, int tok, int k0) {
+    if (k0 <= -32) {
+        return 0xffffffffu;
+    }
+    if (mask == nullptr) { // a chain: up to the token itself
+        const int n = tok - k0 + 1;
+        return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+    }
+    if (k0 < 0) {
+        return (mask[0] << -k0) | ((1u << -k0) - 1u);
+    }
+    const int w = k0 >> 5, s = k0 & 31;
+    const uint32_t lo = w < words ? mask[w] : 0u, hi = w + 1 < words ? mask[w + 1] : 0u;
+    return __funnelshift_r(lo, hi, s);
+}
+
+struct TcArgs {
+    TreeAttnArgs a;
+    int group;
+    int box; // places of a TMA box: min(block_size, 128)
+    float* part_o;
+    float2* part_ml;
+    uint32_t* tickets;
+    long long bound;
+};
+
+template <int DP, int kTiles>
+struct TcShape {
+    static constexpr int RT = kTile * kTiles;
+    static constexpr int kSlabs = DP / 64;
+    static constexpr int kSlab = kTile * 128;         // bytes of 64 elements x 128 places
+    static constexpr int kKV = kSlabs * kSlab;        // a K or a V tile
+    static constexpr int kQ = kTiles * kKV;
+    static constexpr int NS = DP == 64 ? 4 : kTiles == 2 ? 2 : 3;
+    static constexpr int kSmem = 1024 + kQ + 2 * NS * kKV;
+};
+
+template <typename T, int DP, int kTiles>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    tree_attn_tc_kernel(const __grid_constant__ TcArgs args, const __grid_constant__ CUtensorMap k_map,
+                        const __grid_constant__ CUtensorMap v_map) {
+    using S = TcShape<DP, kTiles>;
+    constexpr int NS = S::NS, RT = S::RT;
+    constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
+    const TreeAttnArgs& a = args.a;
+    const nb2_tree_attn_geom& g = a.g;
+    extern __shared__ uint8_t tc_dyn[];
+    uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tc_dyn) + 1023) & ~uintptr_t(1023));
+    uint8_t* ks = qs + S::kQ;
+    uint8_t* vs = ks + NS * S::kKV;
+    __shared__ uint64_t k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], s_full[2], p_full[2], o_done[2], q_full, drain;
+    __shared__ int64_t red[kTcThreads / 32], found[2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_word, is_last, hole_word;
+    // of a tile that is prepared (two of them: a thread can be one tile ahead): places that are there, by group, and
+    // places whose values are not finite, by group (0 where both share the tile) and slab
+    __shared__ uint32_t valid_of[2][2][4], odd[2][2][2][4];
+    __shared__ float2 other_ml[kTile];
+    volatile int* abort_flag = &abort_word;
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int group = args.group;
+    bool bad = false;
+    if (tid == 0) {
+        for (int i = 0; i < NS; ++i) {
+            mbar_init(&k_full[i], 1);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_full[i], 1);
+            mbar_init(&v_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], kTile);
+            mbar_init(&o_done[i], 1);
+        }
+        mbar_init(&q_full, kSoftmax);
+        mbar_init(&drain, 1);
+        abort_word = 0;
+        hole_word = 0;
+        fence_mbar_init();
+    }
+    if (warp == 9) {
+        tmem_alloc(&tmem_slot, 512);
+        tmem_relinquish();
+    }
+    if (warp == 8 && lane == 0) {
+        prefetch_tmap(&k_map);
+        prefetch_tmap(&v_map);
+    }
+    const Span span = find_span<RT, kTile, kTcThreads>(a, group, red, found, bad);
+    spare_tokens<T>(a, tid, kTcThreads);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    // every role walks the same items
+    auto items = [&](auto&& body) {
+        int r = span.request;
+        int64_t r_unit = span.request_unit;
+        Request rq{};
+        if (span.w0 < span.w1) {
+            rq = request_at<RT, kTile>(a, r, group);
+        }
+        for (int64_t w = span.w0; w < span.w1;) {
+            while (w >= r_unit + rq.units(g.kv_heads)) {
+                r_unit += rq.units(g.kv_heads);
+                rq = request_at<RT, kTile>(a, ++r, group);
+            }
+            const int64_t item = (w - r_unit) / rq.tiles, item_w0 = r_unit + item * rq.tiles;
+            const int kvh = static_cast<int>(item / rq.row_blocks);
+            const int rb = static_cast<int>(item - static_cast<int64_t>(kvh) * rq.row_blocks);
+            const int t0 = static_cast<int>(w - item_w0);
+            const int t1 = static_cast<int>(min(span.w1, item_w0 + rq.tiles) - item_w0);
+            body(r, rq, item_w0, kvh, rb, t0, t1);
+            w = item_w0 + t1;
+        }
+    };
+
+    if (warp == 8) {
+        // ---- TMA: a lane a box
+        uint32_t n = 0; // tiles so far
+        const int size = static_cast<int>(g.block_size), boxes = kTile / args.box;
+        items([&](int r, const Request& rq, int64_t, int kvh, int, int t0, int t1) {
+            const int32_t* table = a.table + r * g.table_stride;
+            for (int t = t0; t < t1; ++t, ++n) {
+                const int st = n % NS;
+                const uint32_t phase = (n / NS + 1) & 1;
+                // 128 places are at most 16 boxes of a slab; lane = box + 16 * slab
+                const int box = lane & 15, slab = lane >> 4;
+                const bool mine = box < boxes && slab < S::kSlabs;
+                const int j = t * kTile + box * args.box;
+                int block = -1; // out of range: zeros
+                if (mine && j < rq.total) {
+                    block = table[j / size];
+                    block = block < 0 || block >= g.num_blocks ? -1 : block;
+                }
+                bool ok = mbar_wait(&k_empty[st], phase, abort_flag, a.err, args.bound);
+                ok = __all_sync(0xffffffffu, ok);
+                if (ok) {
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&k_full[st], S::kKV);
+                    }
+                    __syncwarp();
+                    if (mine) {
+                        tma_load_page(ks + st * S::kKV + slab * S::kSlab + box * args.box * 128, &k_map, slab * 64, kvh,
+                                      j % size, block, &k_full[st]);
+                    }
+                }
+                ok = mbar_wait(&v_empty[st], phase, abort_flag, a.err, args.bound);
+                ok = __all_sync(0xffffffffu, ok);
+                if (ok) {
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&v_full[st], S::kKV);
+                    }
+                    __syncwarp();
+                    if (mine) {
+                        tma_load_page(vs + st * S::kKV + slab * S::kSlab + box * args.box * 128, &v_map, slab * 64, kvh,
+                                      j % size, block, &v_full[st]);
+                    }
+                }
+            }
+        });
+        // copies in flight land before the CTA may go: their barriers complete on their own
+        for (uint32_t i = n > NS ? n - NS : 0; i < n; ++i) {
+            const long long c0 = clock64();
+            while (!mbar_try_wait(&k_full[i % NS], (i / NS) & 1) && clock64() - c0 < kWaitBoundCycles && !*abort_flag) {
+            }
+            while (!mbar_try_wait(&v_full[i % NS], (i / NS) & 1) && clock64() - c0 < kWaitBoundCycles && !*abort_flag) {
+            }
+        }
+        if (*abort_flag) { // some barriers will not complete: give the copies the time they take
+            const long long c0 = clock64();
+            while (clock64() - c0 < 2000000) {
+            }
+        }
+    } else if (warp == 9) {
+        // ---- MMA: one thread
+        if (lane == 0) {
+            uint32_t n = 0, q_uses = 0;      // tiles, items so far
+            uint32_t p_uses[2] = {0, 0};     // P tiles taken of each group, as many products O
+            const uint32_t idesc_s = idesc_f16(kBf16, kTile, false), idesc_o = idesc_f16(kBf16, DP, true);
+            auto wait = [&](uint64_t* bar, uint32_t parity) {
+                const bool ok = mbar_wait(bar, parity, abort_flag, a.err, args.bound);
+                tc_fence_after();
+                return ok;
+            };
+            auto scores = [&](int s, uint32_t tile) { // S_s = Q K^T
+                const uint32_t q = smem_u32(qs + (kTiles == 2 ? s * S::kKV : 0)), k = smem_u32(ks + (tile % NS) * S::kKV);
+#pragma unroll
+                for (int i = 0; i < DP / 16; ++i) {
+                    const uint32_t at = (i / 4) * S::kSlab + (i % 4) * 32;
+                    mma_f16(tmem + s * kTile, sdesc_128(q + at, 16), sdesc_128(k + at, 16), idesc_s, i > 0);
+                }
+                mma_commit(&s_full[s]);
+            };
+            auto output = [&](int s, uint32_t tile) { // O_s += P_s V
+                const uint32_t v = smem_u32(vs + (tile % NS) * S::kKV);
+#pragma unroll
+                for (int i = 0; i < kTile / 16; ++i) {
+                    mma_f16_ta(tmem + kColO + s * kTile, tmem + s * kTile + i * 8, sdesc_128(v + i * 2048, S::kSlab),
+                               idesc_o);
+                }
+                mma_commit(&o_done[s]);
+            };
+            items([&](int, const Request&, int64_t, int, int, int t0, int t1) {
+                const int nt = t1 - t0;
+                bool ok = wait(&q_full, q_uses & 1);
+                ++q_uses;
+                // first scores of both groups
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const int i = kTiles == 2 ? 0 : s;
+                    if (i < nt) {
+                        ok = ok && wait(&k_full[(n + i) % NS], ((n + i) / NS) & 1);
+                        if (ok) {
+                            scores(s, n + i);
+                            if (kTiles == 1 || s == 1) {
+                                mma_commit(&k_empty[(n + i) % NS]);
+                            }
+                        }
+                    }
+                }
+                for (int i = 0; i < nt; ++i) {
+                    const uint32_t tile = n + i;
+                    ok = ok && wait(&v_full[tile % NS], (tile / NS) & 1);
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        if (kTiles == 1 && s != (i & 1)) {
+                            continue;
+                        }
+                        ok = ok && wait(&p_full[s], p_uses[s] & 1);
+                        if (ok) {
+                            output(s, tile);
+                            if (kTiles == 1 || s == 1) {
+                                mma_commit(&v_empty[tile % NS]);
+                            }
+                        }
+                        const int next = i + (kTiles == 2 ? 1 : 2);
+                        if (next < nt) {
+                            // the scores go where the weights that this product reads lie
+                            ok = ok && wait(&k_full[(n + next) % NS], ((n + next) / NS) & 1);
+                            ok = ok && wait(&o_done[s], p_uses[s] & 1);
+                            if (ok) {
+                                scores(s, n + next);
+                                if (kTiles == 1 || s == 1) {
+                                    mma_commit(&k_empty[(n + next) % NS]);
+                                }
+                            }
+                        }
+                        ++p_uses[s];
+                    }
+                }
+                n += nt;
+            });
+            // what was issued completes before tensor memory is freed
+            mma_commit(&drain);
+            const long long c0 = clock64();
+            while (!mbar_try_wait(&drain, 0) && clock64() - c0 < kWaitBoundCycles) {
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- softmax: group s, one row a thread
+        const int s = warp >> 2, wt = tid & 127;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t t_s = tmem + lanes + s * kTile, t_o = tmem + lanes + kColO + s * kTile;
+        const float scale2 = fmaxf(fabsf(g.scale) * kLog2e, 1e-30f); // not 0: -inf * 0 is no weight
+        const bool flip = g.scale < 0.0f; // Q is negated instead, so that a row's largest product is its maximum
+        const int size = static_cast<int>(g.block_size);
+        const int share = kTiles == 2 ? kSoftmax : kTile; // threads that prepare a tile together
+        uint32_t s_uses = 0, n = 0;
+        uint32_t zeros[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            zeros[i] = 0;
+        }
+        items([&](int r, const Request& rq, int64_t item_w0, int kvh, int rb, int t0, int t1) {
+            const int rows = min(RT, rq.n * group - rb * RT);
+            const int old = rq.total - rq.n;
+            const int32_t* table = a.table + r * g.table_stride;
+            const int row = (kTiles == 2 ? s * kTile : 0) + wt;
+            const int tok = row < rows ? (rb * RT + row) / group : -1;
+            const uint32_t* mask = a.mask != nullptr ? a.mask + (rq.first + max(tok, 0)) * g.mask_words : nullptr;
+            // ---- Q into shared memory (K-major slabs of 64), zero past the rows and head_dim
+            for (int i = tid; i < RT * DP / 8; i += kSoftmax) {
+                const int qr = i / (DP / 8), ch = i - qr * (DP / 8);
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (qr < rows && ch * 8 < g.head_dim) {
+                    const int rho = rb * RT + qr, qt = rho / group;
+                    const int64_t h = static_cast<int64_t>(kvh) * group + (rho - qt * group);
+                    x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (rq.first + qt) * g.q_stride +
+                                                        h * g.q_head_stride + ch * 8);
+                }
+                if (flip) {
+                    x.x ^= 0x80008000u, x.y ^= 0x80008000u, x.z ^= 0x80008000u, x.w ^= 0x80008000u;
+                }
+                uint8_t* slab = qs + (qr / kTile) * S::kKV + (ch / 8) * S::kSlab;
+                const int lr = qr % kTile;
+                *reinterpret_cast<uint4*>(slab + lr * 128 + (((ch & 7) ^ (lr & 7)) << 4)) = x;
+            }
+            // places of this CTA's tiles without a block: then every tile looks its places up
+            bool hole = false;
+            for (int j = t0 * kTile / size + tid; j * static_cast<int64_t>(size) < min(rq.total, t1 * kTile); j += kSoftmax) {
+                hole |= table[j] < 0 || table[j] >= g.num_blocks;
+            }
+            if (hole) {
+                hole_word = 1;
+                bad = true;
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&q_full);
+#pragma unroll
+            for (int c = 0; c < DP; c += 32) {
+                tmem_st32(t_o + c, zeros);
+            }
+            tmem_wait_st();
+            bar_named(1, kSoftmax);
+            const bool holes = *const_cast<volatile int*>(&hole_word) != 0;
+
+            float m = -INFINITY, z = 0.0f; // reference and sum of this row
+            bool ok = !*abort_flag;
+            for (int t = t0 + (kTiles == 2 ? 0 : s); t < t1; t += kTiles == 2 ? 1 : 2) {
+                const uint32_t tile = n + (t - t0);
+                const int j0 = t * kTile;
+                const bool plain = j0 + kTile <= old && !holes;
+                uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+                const int mine = kTiles == 2 ? 0 : s; // whose odd[] the tile uses
+                if (!plain) {
+                    // ---- V's rows that may not be multiplied: no such place, or not finite
+                    uint8_t* vt = vs + (tile % NS) * S::kKV;
+                    const int j = j0 + wt; // the place of this thread
+                    bool there = j < rq.total;
+                    if (there && holes) {
+                        const int b = table[j / size];
+                        there = b >= 0 && b < g.num_blocks;
+                    }
+                    const uint32_t valid = __ballot_sync(0xffffffffu, there);
+                    ok = mbar_wait(&v_full[tile % NS], (tile / NS) & 1, abort_flag, a.err, args.bound) && ok;
+#pragma unroll
+                    for (int sl = 0; sl < S::kSlabs; ++sl) {
+                        if (kTiles == 2 && S::kSlabs == 2 && sl != s) {
+                            continue; // the groups share the slabs
+                        }
+                        if (kTiles == 2 && S::kSlabs == 1 && s != 0) {
+                            continue;
+                        }
+                        uint8_t* vr = vt + sl * S::kSlab + wt * 128;
+                        bool odd_here = false;
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {
+                            const uint4 x = *reinterpret_cast<const uint4*>(vr + c * 16);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const uint32_t u = e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w;
+                                constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u;
+                                odd_here |= (u & kExp) == kExp || ((u >> 16) & kExp) == kExp;
+                            }
+                        }
+                        if (!there || odd_here) {
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) {
+                                *reinterpret_cast<uint4*>(vr + c * 16) = make_uint4(0, 0, 0, 0);
+                            }
+                        }
+                        const uint32_t o = __ballot_sync(0xffffffffu, there && odd_here);
+                        if (lane == 0) {
+                            odd[s_uses & 1][mine][sl][warp & 3] = o;
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    if (lane == 0) {
+                        valid_of[s_uses & 1][s][warp & 3] = valid;
+                    }
+                    bar_named(kTiles == 2 ? 1 : 2 + s, share);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        see[w] = tok < 0 ? 0u
+                                         : valid_of[s_uses & 1][s][w] &
+                                               see_bits(mask, g.mask_words, tok, j0 + 32 * w - old);
+                    }
+                }
+                // ---- the row's scores
+                ok = mbar_wait(&s_full[s], s_uses & 1, abort_flag, a.err, args.bound) && ok;
+                __syncwarp();
+                tc_fence_after();
+                auto chunk = [&](int c, float (&x)[32]) {
+                    uint32_t v[32];
+                    tmem_ld32(t_s + c * 32, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        x[i] = __uint_as_float(v[i]);
+                    }
+                    if (!plain) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            x[i] = (see[c] >> i) & 1u ? x[i] : -INFINITY;
+                        }
+                    }
+                };
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float x[32];
+                    chunk(c, x);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        top[i & 3] = fmaxf(top[i & 3], x[i]);
+                    }
+                }
+                // -inf stays -inf whatever the scale (0 * -inf would not)
+                const float raw = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                const float now = raw == -INFINITY ? -INFINITY : raw * scale2;
+                if (__any_sync(0xffffffffu, now > m + 8.0f)) {
+                    const float to = fmaxf(m, now), keep = to == -INFINITY ? 1.0f : exp2_fast(m - to);
+                    if (__any_sync(0xffffffffu, m > -INFINITY)) { // O is at rest: this tile's scores were made after it
+                        for (int c = 0; c < DP; c += 32) {
+                            uint32_t v[32];
+                            tmem_ld32(t_o + c, v);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                v[i] = __float_as_uint(__uint_as_float(v[i]) * keep);
+                            }
+                            tmem_st32(t_o + c, v);
+                        }
+                        tmem_wait_st();
+                    }
+                    z *= keep;
+                    m = to;
+                }
+                const float ref = m == -INFINITY ? 0.0f : m;
+                if (!plain) {
+                    // ---- places whose values are not finite, for the rows that see them
+#pragma unroll 1
+                    for (int sw = 0; sw < S::kSlabs * 4; ++sw) {
+                        const int sl = sw >> 2, w = sw & 3;
+                        for (uint32_t left = odd[s_uses & 1][mine][sl][w]; left != 0; left &= left - 1) {
+                            const int key = w * 32 + __ffs(left) - 1, j = j0 + key;
+                            uint32_t raw_s;
+                            tmem_ld1(t_s + key, raw_s);
+                            tmem_wait_ld();
+                            const bool sees = (see[0] >> (key & 31) & 1u & (w == 0)) | (see[1] >> (key & 31) & 1u & (w == 1)) |
+                                              (see[2] >> (key & 31) & 1u & (w == 2)) | (see[3] >> (key & 31) & 1u & (w == 3));
+                            const float p = sees ? exp2_fast(fmaf(__uint_as_float(raw_s), scale2, -ref)) : 0.0f;
+                            const int64_t b = table[j / size];
+                            const T* v = static_cast<const T*>(a.vc) + b * g.vc_block_stride + (j % size) * g.vc_place_stride +
+                                         kvh * g.vc_head_stride + sl * 64;
+                            for (int c = 0; c < 64; c += 32) {
+                                uint32_t o[32];
+                                tmem_ld32(t_o + sl * 64 + c, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) {
+                                    const bool in = sl * 64 + c + i < g.head_dim;
+                                    const float f = in ? to_f32(v[in ? c + i : 0]) : 0.0f;
+                                    o[i] = p > 0.0f ? __float_as_uint(__uint_as_float(o[i]) + p * f) : o[i];
+                                }
+                                tmem_st32(t_o + sl * 64 + c, o);
+                                tmem_wait_st();
+                            }
+                        }
+                    }
+                }
+                // ---- weights, packed over the scores; their sum keeps all bits
+                float zz[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float x[32];
+                    chunk(c, x);
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float p0 = exp2_fast(fmaf(x[2 * i], scale2, -ref));
+                        const float p1 = exp2_fast(fmaf(x[2 * i + 1], scale2, -ref));
+                        zz[(2 * i) & 3] += p0;
+                        zz[(2 * i + 1) & 3] += p1;
+                        pk[i] = pack2<T>(p0, p1);
+                    }
+                    tmem_st16u(t_s + c * 16, pk);
+                }
+                z += (zz[0] + zz[1]) + (zz[2] + zz[3]);
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(&p_full[s]);
+                ++s_uses;
+            }
+            // ---- the item's end: O at rest, joined where the groups share rows, stored
+            const int my_tiles = kTiles == 2 ? t1 - t0 : (t1 - t0 + 1 - s) / 2;
+            if (my_tiles > 0) {
+                // s_uses counts this group's tiles, each with one product
+                ok = mbar_wait(&o_done[s], (s_uses - 1) & 1, abort_flag, a.err, args.bound) && ok;
+            }
+            __syncwarp();
+            tc_fence_after();
+            const bool whole = t0 == 0 && t1 == rq.tiles;
+            const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0);
+            float mm = m, ff = 1.0f, f_other = 0.0f, zs = z;
+            if (kTiles == 1) {
+                // both groups hold all rows' sums over half of the tiles: each joins half of the elements
+                if (s == 1) {
+                    other_ml[wt] = make_float2(m, z);
+                }
+                tc_fence_before();
+                bar_named(1, kSoftmax);
+                tc_fence_after();
+                const float2 o1 = other_ml[wt];
+                bar_named(1, kSoftmax);
+                if (s == 0) {
+                    other_ml[wt] = make_float2(m, z);
+                }
+                bar_named(1, kSoftmax);
+                const float2 o2 = other_ml[wt];
+                const float2 ot = s == 0 ? o1 : o2;
+                mm = fmaxf(m, ot.x);
+                const float ref = mm == -INFINITY ? 0.0f : mm;
+                ff = exp2_fast(m - ref);
+                f_other = exp2_fast(ot.x - ref);
+                // the same order in both groups
+                zs = s == 0 ? ff * z + f_other * ot.y : f_other * ot.y + ff * z;
+            }
+            const bool live = row < rows && ok && !*abort_flag;
+            constexpr int kCols = kTiles == 2 ? DP : DP / 2;
+            const int c0 = kTiles == 2 ? 0 : s * kCols;
+            const int rho = rb * RT + row;
+            const int64_t tk = rq.first + max(tok, 0), h = static_cast<int64_t>(kvh) * group + (rho - max(tok, 0) * group);
+            const float inv = 1.0f / zs;
+            const bool none = zs == 0.0f;
+#pragma unroll
+            for (int c = 0; c < kCols; c += 32) {
+                uint32_t v[32];
+                __syncwarp();
+                tmem_ld32(t_o + c0 + c, v);
+                tmem_wait_ld();
+                if (kTiles == 1) {
+                    uint32_t u[32];
+                    tmem_ld32(tmem + lanes + kColO + (1 - s) * kTile + c0 + c, u);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const float p = ff != 0.0f ? ff * __uint_as_float(v[i]) : 0.0f;
+                        const float q = f_other != 0.0f ? f_other * __uint_as_float(u[i]) : 0.0f;
+                        v[i] = __float_as_uint(s == 0 ? p + q : q + p);
+                    }
+                }
+                if (live && whole) {
+                    T* out = static_cast<T*>(a.out) + tk * g.o_stride + h * g.o_head_stride + c0 + c;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        if (c0 + c + i < g.head_dim) {
+                            uint32_t y[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                y[e] = none ? 0u
+                                            : pack2<T>(__uint_as_float(v[i + 2 * e]) * inv, __uint_as_float(v[i + 2 * e + 1]) * inv);
+                            }
+                            *reinterpret_cast<uint4*>(out + i) = make_uint4(y[0], y[1], y[2], y[3]);
+                        }
+                    }
+                } else if (live) {
+                    uint4* o = reinterpret_cast<uint4*>(args.part_o + (slot * RT + row) * DP + c0 + c);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        o[i / 4] = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                    }
+                }
+            }
+            if (live && (kTiles == 2 || s == 0)) {
+                if (!whole) {
+                    args.part_ml[slot * RT + row] = make_float2(mm, zs);
+                } else if (a.lse != nullptr) {
+                    a.lse[tk * g.q_heads + h] = none ? -INFINITY : mm * kLn2 + logf(zs);
+                }
+            }
+            if (!whole) {
+                const int p0 = cta_of(item_w0, span.W, span.grid), p1 = cta_of(item_w0 + rq.tiles - 1, span.W, span.grid);
+                __threadfence();
+                bar_named(1, kSoftmax);
+                if (tid == 0) {
+                    const uint32_t k = atomicAdd(&args.tickets[p0], 1u);
+                    is_last = k == static_cast<uint32_t>(p1 - p0);
+                    if (is_last) {
+                        args.tickets[p0] = 0; // for the next launch
+                    }
+                }
+                bar_named(1, kSoftmax);
+                if (*const_cast<volatile int*>(&is_last)) {
+                    __threadfence();
+                    join_pieces<T, DP, RT, kSoftmax>(a, args.part_o, args.part_ml, p0, p1, rq.first, kvh, group, rb * RT,
+                                                     rows, tid);
+                }
+            }
+            tc_fence_before();
+            bar_named(1, kSoftmax); // shared words and Q are free for the next item
+            if (tid == 0) {
+                hole_word = 0;
+            }
+            bar_named(1, kSoftmax);
+            n += t1 - t0;
+        });
+    }
+    if (bad) {
+        record_error(a.err, kDevIndexOutOfRange);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+CUtensorMap page_map(const void* base, const nb2_tree_attn_geom& g, bool bf16, int64_t block_stride, int64_t place_stride,
+                     int64_t head_stride, int box) {
+    CUtensorMap m{};
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(g.head_dim), static_cast<cuuint64_t>(g.kv_heads),
+                                static_cast<cuuint64_t>(g.block_size), static_cast<cuuint64_t>(g.num_blocks)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(head_stride * 2), static_cast<cuuint64_t>(place_stride * 2),
+                                   static_cast<cuuint64_t>(block_stride * 2)};
+    const cuuint32_t boxes[4] = {64, 1, static_cast<cuuint32_t>(box), 1}, ones[4] = {1, 1, 1, 1};
+    const CUresult e = encode_tiled()(&m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                                      const_cast<void*>(base), dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (e != CUDA_SUCCESS) {
+        fail(kStatusCuda, "tree attention: cuTensorMapEncodeTiled failed (" + std::to_string(static_cast<int>(e)) + ")");
+    }
+    return m;
+}
+
+template <typename T, int DP, int kTiles>
+void launch_tc(nb2_device* dev, const TreeAttnArgs& a) {
+    using S = TcShape<DP, kTiles>;
+    auto kernel = tree_attn_tc_kernel<T, DP, kTiles>;
+    static bool set[64] = {};
+    if (!set[dev->ordinal]) {
+        check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem),
+                   "cudaFuncSetAttribute(tree attention)");
+        set[dev->ordinal] = true;
+    }
+    const nb2_tree_attn_geom& g = a.g;
+    constexpr bool bf16 = std::is_same_v<T, __nv_bfloat16>;
+    const int box = static_cast<int>(std::min<int64_t>(g.block_size, kTile));
+    const CUtensorMap km = page_map(a.kc, g, bf16, g.kc_block_stride, g.kc_place_stride, g.kc_head_stride, box);
+    const CUtensorMap vm = page_map(a.vc, g, bf16, g.vc_block_stride, g.vc_place_stride, g.vc_head_stride, box);
+    const int grid = dev->num_sms;
+    const size_t o_bytes = static_cast<size_t>(grid) * 2 * S::RT * DP * 4;
+    uint8_t* ws = static_cast<uint8_t*>(dev->scratch(o_bytes + static_cast<size_t>(grid) * 2 * S::RT * 8));
+    TcArgs args{a, static_cast<int>(g.q_heads / g.kv_heads), box, reinterpret_cast<float*>(ws),
+                reinterpret_cast<float2*>(ws + o_bytes), dev->tickets(grid), dev->wait_bound};
+    kernel<<<grid, kTcThreads, S::kSmem, dev->stream>>>(args, km, vm);
+    check_cuda(cudaGetLastError(), "tree attention launch");
+}
+
+template <typename T, int DP>
+void pick_tiles(nb2_device* dev, const TreeAttnArgs& a) {
+    const int64_t rows = std::min(a.g.max_new, a.g.tokens) * (a.g.q_heads / a.g.kv_heads);
+    rows > kTile ? launch_tc<T, DP, 2>(dev, a) : launch_tc<T, DP, 1>(dev, a);
+}
+
+} // namespace
+
+bool tree_attention_tc_takes(const TreeAttnArgs& a) {
+    const nb2_tree_attn_geom& g = a.g;
+    const int64_t rows = std::min(g.max_new, g.tokens) * (g.q_heads / g.kv_heads);
+    const bool page = g.block_size >= 8 && (g.block_size & (g.block_size - 1)) == 0;
+    const int64_t most = int64_t{1} << 39; // a map's stride, in elements here
+    bool strides = true;
+    for (int64_t s : {g.kc_block_stride, g.kc_place_stride, g.kc_head_stride, g.vc_block_stride, g.vc_place_stride,
+                      g.vc_head_stride}) {
+        strides = strides && s > 0 && s < most;
+    }
+    return g.dtype != kF32 && rows > kTcRows && g.head_dim >= 64 && g.head_dim <= 128 && page && strides && g.num_blocks > 0;
+}
+
+void tree_attention_tc(nb2_device* dev, const TreeAttnArgs& a) {
+    if (a.g.dtype == kF16) {
+        a.g.head_dim <= 64 ? pick_tiles<__half, 64>(dev, a) : pick_tiles<__half, 128>(dev, a);
+    } else {
+        a.g.head_dim <= 64 ? pick_tiles<__nv_bfloat16, 64>(dev, a) : pick_tiles<__nv_bfloat16, 128>(dev, a);
+    }
+}
+
+} // namespace nb2
