@@ -143,18 +143,23 @@ __global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(TreeAttnArgs a,
     if (span.w0 < w1) {
         rq = request_at<RT, KT>(a, r, group);
     }
-    for (int64_t w = span.w0; w < w1;) {
+    for (int64_t w = span.w0; w < w1;) { // w: the first unit not yet looked at
         while (w >= r_unit + rq.units(g.kv_heads)) {
             r_unit += rq.units(g.kv_heads);
             rq = request_at<RT, KT>(a, ++r, group);
         }
         // ---- the item and this CTA's tiles of it
-        const int64_t item = (w - r_unit) / rq.tiles;
-        const int64_t item_w0 = r_unit + item * rq.tiles, item_w1 = item_w0 + rq.tiles;
+        const int64_t item = (w - r_unit) / rq.per_item();
+        const int64_t item_w0 = r_unit + item * rq.per_item() + Request::kExtra, item_w1 = item_w0 + rq.tiles;
+        const int64_t from = max(w, item_w0);
+        w = min(w1, item_w1);
+        if (from >= w) {
+            continue; // the span ends before the item's first tile
+        }
         const int64_t kvh = item / rq.row_blocks;
         const int rb = static_cast<int>(item - kvh * rq.row_blocks);
-        const int t_begin = static_cast<int>(w - item_w0);
-        const int t_end = static_cast<int>(min(w1, item_w1) - item_w0);
+        const int t_begin = static_cast<int>(from - item_w0);
+        const int t_end = static_cast<int>(w - item_w0);
         const int rows = min(RT, rq.n * group - rb * RT);
         const int old = rq.total - rq.n; // -n where the lengths are wrong: then total is 0 and no place is seen
         const int32_t* table = a.table + r * g.table_stride;
@@ -582,7 +587,6 @@ __global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(TreeAttnArgs a,
                 join_pieces<T, DP, RT, NT>(a, part_o, part_ml, c0, c1, rq.first, kvh, group, rb * RT, rows, tid);
             }
         }
-        w = item_w0 + t_end;
     }
     if (bad) {
         record_error(a.err, kDevIndexOutOfRange);

@@ -17,8 +17,11 @@ struct Request {
     int row_blocks; // blocks of its n * group rows
     int tiles;      // tiles of its places, at least one so that rows without places are written
     bool bad;
+    // What beginning and ending an item costs a CTA, in tiles: Q, the pipeline's fill, the stores and the join.
+    static constexpr int kExtra = 2;
+    __device__ __forceinline__ int per_item() const { return tiles + kExtra; }
     __device__ __forceinline__ int64_t units(int64_t kv_heads) const {
-        return static_cast<int64_t>(row_blocks) * kv_heads * tiles;
+        return static_cast<int64_t>(row_blocks) * kv_heads * per_item();
     }
 };
 
@@ -99,29 +102,53 @@ __device__ __forceinline__ void store_row4(const TreeAttnArgs& a, int64_t first,
 template <typename T, int DP, int RT, int NT>
 __device__ __forceinline__ void join_pieces(const TreeAttnArgs& a, const float* part_o, const float2* part_ml, int c0, int c1,
                                             int64_t first, int64_t kvh, int group, int rho0, int rows, int tid) {
-    for (int i = tid; i < rows * (DP / 4); i += NT) {
-        const int row = i / (DP / 4), d = (i - row * (DP / 4)) * 4;
-        if (d >= a.g.head_dim) {
-            continue;
+    // kAhead elements of a thread at a time: one after another, the loads of a piece took longer than its tiles
+    constexpr int kAhead = 8;
+    for (int i0 = tid; i0 < rows * (DP / 4); i0 += kAhead * NT) {
+        float m[kAhead], z[kAhead];
+        float4 x[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            m[u] = -INFINITY;
+            z[u] = 0.0f;
+            x[u] = make_float4(0, 0, 0, 0);
         }
-        float m = -INFINITY;
-        for (int c = c0; c <= c1; ++c) {
-            m = fmaxf(m, __ldcg(&part_ml[(2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0)) * RT + row]).x);
-        }
-        const float ref = m == -INFINITY ? 0.0f : m;
-        float z = 0.0f;
-        float4 x = make_float4(0, 0, 0, 0);
         for (int c = c0; c <= c1; ++c) {
             const int64_t slot = 2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0);
-            const float2 ml = __ldcg(&part_ml[slot * RT + row]);
-            const float f = exp2_fast(ml.x - ref);
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(part_o + (slot * RT + row) * DP + d));
-            z += f * ml.y;
-            if (f != 0.0f) { // a piece that saw nothing adds nothing
-                x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
+            float2 ml[kAhead];
+            float4 y[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int i = i0 + u * NT, row = i / (DP / 4), d = (i - row * (DP / 4)) * 4;
+                if (row < rows && d < a.g.head_dim) {
+                    ml[u] = __ldcg(&part_ml[slot * RT + row]);
+                    y[u] = __ldcg(reinterpret_cast<const float4*>(part_o + (slot * RT + row) * DP + d));
+                } else {
+                    ml[u] = make_float2(-INFINITY, 0.0f);
+                    y[u] = make_float4(0, 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const float to = fmaxf(m[u], ml[u].x), ref = to == -INFINITY ? 0.0f : to;
+                const float f = exp2_fast(m[u] - ref), h = exp2_fast(ml[u].x - ref);
+                m[u] = to;
+                z[u] = f * z[u] + h * ml[u].y;
+                if (h != 0.0f) { // a piece that saw nothing adds nothing
+                    x[u].x = f * x[u].x + h * y[u].x;
+                    x[u].y = f * x[u].y + h * y[u].y;
+                    x[u].z = f * x[u].z + h * y[u].z;
+                    x[u].w = f * x[u].w + h * y[u].w;
+                }
             }
         }
-        store_row4<T>(a, first, kvh, group, rho0 + row, d, x, m, z);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int i = i0 + u * NT, row = i / (DP / 4), d = (i - row * (DP / 4)) * 4;
+            if (row < rows && d < a.g.head_dim) {
+                store_row4<T>(a, first, kvh, group, rho0 + row, d, x[u], m[u], z[u]);
+            }
+        }
     }
 }
 
@@ -159,13 +186,14 @@ __device__ __forceinline__ Span find_span(const TreeAttnArgs& a, int group, int6
     const int B = static_cast<int>(a.g.batch);
     const int64_t cta = blockIdx.x;
     Span s{};
-    int64_t sum = 0;
+    int64_t mine = 0; // units of request tid
     for (int r = tid; r < B; r += NT) {
         const Request q = request_at<RT, KT>(a, r, group);
         bad |= q.bad;
-        sum += q.units(a.g.kv_heads);
+        s.W += q.units(a.g.kv_heads);
+        mine = r == tid ? s.W : mine;
     }
-    s.W = block_sum<NT>(sum, red);
+    s.W = block_sum<NT>(s.W, red);
     s.grid = min(static_cast<int64_t>(gridDim.x), s.W); // no span is empty
     if (cta >= s.grid) {
         return s;
@@ -174,7 +202,7 @@ __device__ __forceinline__ Span find_span(const TreeAttnArgs& a, int group, int6
     s.w1 = (cta + 1) * s.W / s.grid;
     int64_t base = 0;
     for (int c = 0; c < B; c += NT) {
-        const int64_t u = c + tid < B ? request_at<RT, KT>(a, c + tid, group).units(a.g.kv_heads) : 0;
+        const int64_t u = c == 0 ? mine : c + tid < B ? request_at<RT, KT>(a, c + tid, group).units(a.g.kv_heads) : 0;
         int64_t inc = u;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {

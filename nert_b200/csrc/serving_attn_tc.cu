@@ -239,13 +239,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 r_unit += rq.units(g.kv_heads);
                 rq = request_at<RT, kTile>(a, ++r, group);
             }
-            const int64_t item = (w - r_unit) / rq.tiles, item_w0 = r_unit + item * rq.tiles;
-            const int kvh = static_cast<int>(item / rq.row_blocks);
-            const int rb = static_cast<int>(item - static_cast<int64_t>(kvh) * rq.row_blocks);
-            const int t0 = static_cast<int>(w - item_w0);
-            const int t1 = static_cast<int>(min(span.w1, item_w0 + rq.tiles) - item_w0);
-            body(r, rq, item_w0, kvh, rb, t0, t1);
-            w = item_w0 + t1;
+            const int64_t item = (w - r_unit) / rq.per_item();
+            const int64_t item_w0 = r_unit + item * rq.per_item() + Request::kExtra; // its first tile
+            const int64_t from = max(w, item_w0);
+            w = min(span.w1, item_w0 + rq.tiles);
+            if (from < w) {
+                const int kvh = static_cast<int>(item / rq.row_blocks);
+                const int rb = static_cast<int>(item - static_cast<int64_t>(kvh) * rq.row_blocks);
+                body(r, rq, item_w0, kvh, rb, static_cast<int>(from - item_w0), static_cast<int>(w - item_w0));
+            }
         }
     };
 
@@ -414,22 +416,44 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int row = (kTiles == 2 ? s * kTile : 0) + wt;
             const int tok = row < rows ? (rb * RT + row) / group : -1;
             const uint32_t* mask = a.mask != nullptr ? a.mask + (rq.first + max(tok, 0)) * g.mask_words : nullptr;
-            // ---- Q into shared memory (K-major slabs of 64), zero past the rows and head_dim
-            for (int i = tid; i < RT * DP / 8; i += kSoftmax) {
-                const int qr = i / (DP / 8), ch = i - qr * (DP / 8);
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (qr < rows && ch * 8 < g.head_dim) {
-                    const int rho = rb * RT + qr, qt = rho / group;
-                    const int64_t h = static_cast<int64_t>(kvh) * group + (rho - qt * group);
-                    x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (rq.first + qt) * g.q_stride +
-                                                        h * g.q_head_stride + ch * 8);
+            // the 16-byte chunks of the item's rows, in q and in out, shared by the 256 threads
+            constexpr int kRowChunks = DP / 8, kRowStep = kSoftmax / kRowChunks, kRowSteps = RT / kRowStep;
+            auto for_rows = [&](auto&& f) {
+                const int ch = tid % kRowChunks;
+                int qr = tid / kRowChunks;
+                int qt = (rb * RT + qr) / group, hq = rb * RT + qr - qt * group;
+                const int dt = kRowStep / group, dh = kRowStep - dt * group;
+#pragma unroll
+                for (int u = 0; u < kRowSteps; ++u) {
+                    const int64_t t = rq.first + qt, h = static_cast<int64_t>(kvh) * group + hq;
+                    f(u, qr, ch, static_cast<const T*>(a.q) + t * g.q_stride + h * g.q_head_stride + ch * 8,
+                      static_cast<T*>(a.out) + t * g.o_stride + h * g.o_head_stride + ch * 8);
+                    qr += kRowStep;
+                    qt += dt;
+                    hq += dh;
+                    if (hq >= group) {
+                        hq -= group;
+                        ++qt;
+                    }
                 }
+            };
+            uint4 q_buf[kRowSteps];
+            // ---- Q into shared memory (K-major slabs of 64), zero past the rows and head_dim
+            for_rows([&](int u, int qr, int ch, const T* src, T*) {
+                q_buf[u] = make_uint4(0, 0, 0, 0);
+                if (qr < rows && ch * 8 < g.head_dim) {
+                    q_buf[u] = *reinterpret_cast<const uint4*>(src);
+                }
+            });
+#pragma unroll
+            for (int u = 0; u < kRowSteps; ++u) {
+                const int qr = tid / kRowChunks + u * kRowStep, ch = tid % kRowChunks, lr = qr % kTile;
+                uint4 x = q_buf[u];
                 if (flip) {
                     x.x ^= 0x80008000u, x.y ^= 0x80008000u, x.z ^= 0x80008000u, x.w ^= 0x80008000u;
                 }
-                uint8_t* slab = qs + (qr / kTile) * S::kKV + (ch / 8) * S::kSlab;
-                const int lr = qr % kTile;
-                *reinterpret_cast<uint4*>(slab + lr * 128 + (((ch & 7) ^ (lr & 7)) << 4)) = x;
+                *reinterpret_cast<uint4*>(qs + (qr / kTile) * S::kKV + (ch / 8) * S::kSlab + lr * 128 +
+                                          (((ch & 7) ^ (lr & 7)) << 4)) = x;
             }
             // places of this CTA's tiles without a block: then every tile looks its places up
             bool hole = false;
@@ -481,7 +505,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         bool odd_here = false;
 #pragma unroll
                         for (int c = 0; c < 8; ++c) {
-                            const uint4 x = *reinterpret_cast<const uint4*>(vr + c * 16);
+                            const uint4 x = *reinterpret_cast<const uint4*>(vr + ((c ^ (wt & 7)) << 4)); // no bank twice
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 const uint32_t u = e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w;
@@ -492,7 +516,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         if (!there || odd_here) {
 #pragma unroll
                             for (int c = 0; c < 8; ++c) {
-                                *reinterpret_cast<uint4*>(vr + c * 16) = make_uint4(0, 0, 0, 0);
+                                *reinterpret_cast<uint4*>(vr + ((c ^ (wt & 7)) << 4)) = make_uint4(0, 0, 0, 0);
                             }
                         }
                         const uint32_t o = __ballot_sync(0xffffffffu, there && odd_here);
@@ -652,60 +676,78 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 // the same order in both groups
                 zs = s == 0 ? ff * z + f_other * ot.y : f_other * ot.y + ff * z;
             }
-            const bool live = row < rows && ok && !*abort_flag;
+            const bool clean = ok && !*abort_flag, live = row < rows && clean;
             constexpr int kCols = kTiles == 2 ? DP : DP / 2;
             const int c0 = kTiles == 2 ? 0 : s * kCols;
-            const int rho = rb * RT + row;
-            const int64_t tk = rq.first + max(tok, 0), h = static_cast<int64_t>(kvh) * group + (rho - max(tok, 0) * group);
-            const float inv = 1.0f / zs;
-            const bool none = zs == 0.0f;
+            // finished values of a row's 32 elements from d on, through Q's shared memory (its products are
+            // done) so that the stores to out are of whole rows: a row a thread, each store met 32 lines
+            auto stage = [&](int d, const float (&x)[32], float sum) {
+                const float inv = 1.0f / sum;
+                const bool none = sum == 0.0f; // no place was seen
 #pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    uint32_t y[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        y[e] = none ? 0u : pack2<T>(x[i + 2 * e] * inv, x[i + 2 * e + 1] * inv);
+                    }
+                    *reinterpret_cast<uint4*>(qs + row * DP * 2 + ((((d + i) >> 3) ^ (row & 7)) << 4)) =
+                        make_uint4(y[0], y[1], y[2], y[3]);
+                }
+            };
+            auto finish = [&](float top, float sum) { // after stage() of all elements
+                bar_named(1, kSoftmax);
+                if (clean) {
+                    for_rows([&](int, int qr, int ch, const T*, T* dst) {
+                        if (qr < rows && ch * 8 < g.head_dim) {
+                            *reinterpret_cast<uint4*>(dst) =
+                                *reinterpret_cast<const uint4*>(qs + qr * DP * 2 + ((ch ^ (qr & 7)) << 4));
+                        }
+                    });
+                    if (row < rows && (kTiles == 2 || s == 0) && a.lse != nullptr) {
+                        const int64_t h = static_cast<int64_t>(kvh) * group + (rb * RT + row - tok * group);
+                        a.lse[(rq.first + tok) * g.q_heads + h] = sum == 0.0f ? -INFINITY : top * kLn2 + logf(sum);
+                    }
+                }
+            };
+            // a piece lies in its slot element by element, the rows together
+            float* piece = args.part_o + slot * DP * RT + row;
+#pragma unroll 1
             for (int c = 0; c < kCols; c += 32) {
                 uint32_t v[32];
+                float x[32];
                 __syncwarp();
                 tmem_ld32(t_o + c0 + c, v);
                 tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    x[i] = __uint_as_float(v[i]);
+                }
                 if (kTiles == 1) {
-                    uint32_t u[32];
-                    tmem_ld32(tmem + lanes + kColO + (1 - s) * kTile + c0 + c, u);
+                    tmem_ld32(tmem + lanes + kColO + (1 - s) * kTile + c0 + c, v);
                     tmem_wait_ld();
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        const float p = ff != 0.0f ? ff * __uint_as_float(v[i]) : 0.0f;
-                        const float q = f_other != 0.0f ? f_other * __uint_as_float(u[i]) : 0.0f;
-                        v[i] = __float_as_uint(s == 0 ? p + q : q + p);
+                        const float p = ff != 0.0f ? ff * x[i] : 0.0f;
+                        const float q = f_other != 0.0f ? f_other * __uint_as_float(v[i]) : 0.0f;
+                        x[i] = p + q;
                     }
                 }
-                if (live && whole) {
-                    T* out = static_cast<T*>(a.out) + tk * g.o_stride + h * g.o_head_stride + c0 + c;
-#pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        if (c0 + c + i < g.head_dim) {
-                            uint32_t y[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                y[e] = none ? 0u
-                                            : pack2<T>(__uint_as_float(v[i + 2 * e]) * inv, __uint_as_float(v[i + 2 * e + 1]) * inv);
-                            }
-                            *reinterpret_cast<uint4*>(out + i) = make_uint4(y[0], y[1], y[2], y[3]);
-                        }
-                    }
+                if (whole) {
+                    stage(c0 + c, x, zs);
                 } else if (live) {
-                    uint4* o = reinterpret_cast<uint4*>(args.part_o + (slot * RT + row) * DP + c0 + c);
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        o[i / 4] = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                    for (int i = 0; i < 32; ++i) {
+                        __stcg(piece + static_cast<int64_t>(c0 + c + i) * RT, x[i]);
                     }
                 }
             }
-            if (live && (kTiles == 2 || s == 0)) {
-                if (!whole) {
-                    args.part_ml[slot * RT + row] = make_float2(mm, zs);
-                } else if (a.lse != nullptr) {
-                    a.lse[tk * g.q_heads + h] = none ? -INFINITY : mm * kLn2 + logf(zs);
+            if (whole) {
+                finish(mm, zs);
+            } else {
+                if (live && (kTiles == 2 || s == 0)) {
+                    __stcg(args.part_ml + slot * RT + row, make_float2(mm, zs));
                 }
-            }
-            if (!whole) {
                 const int p0 = cta_of(item_w0, span.W, span.grid), p1 = cta_of(item_w0 + rq.tiles - 1, span.W, span.grid);
                 __threadfence();
                 bar_named(1, kSoftmax);
@@ -718,9 +760,44 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 bar_named(1, kSoftmax);
                 if (*const_cast<volatile int*>(&is_last)) {
+                    // all pieces are there: added in the order of their CTAs
                     __threadfence();
-                    join_pieces<T, DP, RT, kSoftmax>(a, args.part_o, args.part_ml, p0, p1, rq.first, kvh, group, rb * RT,
-                                                     rows, tid);
+                    float top = -INFINITY, sum = 0.0f;
+#pragma unroll 1
+                    for (int c = 0; c < kCols; c += 32) {
+                        float x[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            x[i] = 0.0f;
+                        }
+                        top = -INFINITY;
+                        sum = 0.0f;
+#pragma unroll 1
+                        for (int p = p0; p <= p1; ++p) {
+                            const int64_t at = 2 * static_cast<int64_t>(p) + (p == p0 ? 1 : 0);
+                            const float* o = args.part_o + at * DP * RT + row;
+                            float y[32];
+                            float2 ml = make_float2(-INFINITY, 0.0f);
+                            if (live) {
+                                ml = __ldcg(args.part_ml + at * RT + row);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) {
+                                    y[i] = __ldcg(o + static_cast<int64_t>(c0 + c + i) * RT);
+                                }
+                            }
+                            const float to = fmaxf(top, ml.x), ref = to == -INFINITY ? 0.0f : to;
+                            const float f = exp2_fast(top - ref), h = exp2_fast(ml.x - ref);
+                            top = to;
+                            sum = f * sum + h * ml.y;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                // a piece that saw nothing adds nothing
+                                x[i] = live && h != 0.0f ? f * x[i] + h * y[i] : f * x[i];
+                            }
+                        }
+                        stage(c0 + c, x, sum);
+                    }
+                    finish(top, sum);
                 }
             }
             tc_fence_before();
