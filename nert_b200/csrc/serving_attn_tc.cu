@@ -4,7 +4,7 @@
 // serving_attn.cu; with 33 rows and more that kernel is bound by its mma.sync and
 // shared-memory rate, this one by exponentials (16 a clock and SM) or by HBM.
 //
-// One CTA an SM, ten warps: two softmax groups of four warps, a TMA warp, an MMA thread. K and V
+// One CTA an SM: two softmax groups of four warps, a TMA warp, an MMA thread for each. K and V
 // tiles of 128 places come page by page as 4-D TMA boxes (64 elements x page) into 128-byte
 // swizzled slabs, through rings of their own. Tensor memory holds two score tiles S (128 rows x 128
 // places, fp32) and two accumulators O; group s owns S and O number s, one row a thread, so a row's
@@ -32,7 +32,7 @@ namespace nb2 {
 
 namespace {
 
-constexpr int kTcThreads = 320;
+constexpr int kTcThreads = 384; // two softmax groups; a TMA warp, two MMA warps and one that only makes up the third group
 constexpr int kSoftmax = 256; // threads of the two softmax groups
 constexpr int kTile = 128;    // places of a tile, rows of a block
 constexpr uint32_t kColO = 256;
@@ -71,10 +71,12 @@ __device__ __forceinline__ void mma_f16_ta(uint32_t d, uint32_t a, uint64_t b, u
                  : "memory");
 }
 
-// 32 lanes x 32 columns to registers; complete with tmem_wait_ld().
+// 32 lanes x 32 columns to registers, complete: the wait is part of the statement, so that nothing that uses them can
+// come before it.
 __device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t (&r)[32]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-                 "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
                    "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
                    "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
@@ -83,9 +85,8 @@ __device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t (&r)[32]) {
                  : "r"(t));
 }
 __device__ __forceinline__ void tmem_ld1(uint32_t t, uint32_t& r) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(t));
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;" : "=r"(r) : "r"(t) : "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void tmem_st32(uint32_t t, const uint32_t (&r)[32]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
@@ -114,8 +115,24 @@ __device__ __forceinline__ void tma_load_page(void* dst, const CUtensorMap* map,
                  : "memory");
 }
 
+// Registers of a warp group: the launch's 168 x 384 go as 208 to each softmax group (a row's 128 scores stay in
+// registers) and 88 to the third.
+template <int N>
+__device__ __forceinline__ void regs_up() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_down() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+static_assert((2 * 208 + 88) * 128 <= 168 * 384, "the groups share what the launch has");
+
 __device__ __forceinline__ void bar_named(int id, int threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+__device__ __forceinline__ void bar_arrive(int id, int threads) {
+    asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
 template <typename T>
@@ -196,9 +213,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (tid == 0) {
         for (int i = 0; i < NS; ++i) {
             mbar_init(&k_full[i], 1);
-            mbar_init(&k_empty[i], 1);
+            mbar_init(&k_empty[i], kTiles);
             mbar_init(&v_full[i], 1);
-            mbar_init(&v_empty[i], 1);
+            mbar_init(&v_empty[i], kTiles);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
@@ -206,7 +223,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_init(&o_done[i], 1);
         }
         mbar_init(&q_full, kSoftmax);
-        mbar_init(&drain, 1);
+        mbar_init(&drain, 2);
         abort_word = 0;
         hole_word = 0;
         fence_mbar_init();
@@ -251,7 +268,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
     };
 
-    if (warp == 8) {
+    if (warp >= 8) {
+        regs_down<88>();
+        if (warp == 8) {
         // ---- TMA: a lane a box
         uint32_t n = 0; // tiles so far
         const int size = static_cast<int>(g.block_size), boxes = kTile / args.box;
@@ -308,84 +327,52 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             while (clock64() - c0 < 2000000) {
             }
         }
-    } else if (warp == 9) {
-        // ---- MMA: one thread
-        if (lane == 0) {
-            uint32_t n = 0, q_uses = 0;      // tiles, items so far
-            uint32_t p_uses[2] = {0, 0};     // P tiles taken of each group, as many products O
+        } else if (warp < 11 && lane == 0) {
+            // ---- MMA: a thread a group. An MMA holds its issuing thread about as long as it runs, so one thread for both groups left the
+            // tensor cores idle while it looked for the next work (attention of 8 long contexts 236 us, with two threads MEASURED).
+            const int s = warp - 9;
+            uint32_t n = 0, items_done = 0, uses = 0; // tiles of all items so far, items, this group's tiles
             const uint32_t idesc_s = idesc_f16(kBf16, kTile, false), idesc_o = idesc_f16(kBf16, DP, true);
+            const uint32_t q = smem_u32(qs + (kTiles == 2 ? s * S::kKV : 0)), t_s = tmem + s * kTile,
+                           t_o = tmem + kColO + s * kTile;
             auto wait = [&](uint64_t* bar, uint32_t parity) {
                 const bool ok = mbar_wait(bar, parity, abort_flag, a.err, args.bound);
                 tc_fence_after();
                 return ok;
             };
-            auto scores = [&](int s, uint32_t tile) { // S_s = Q K^T
-                const uint32_t q = smem_u32(qs + (kTiles == 2 ? s * S::kKV : 0)), k = smem_u32(ks + (tile % NS) * S::kKV);
-#pragma unroll
-                for (int i = 0; i < DP / 16; ++i) {
-                    const uint32_t at = (i / 4) * S::kSlab + (i % 4) * 32;
-                    mma_f16(tmem + s * kTile, sdesc_128(q + at, 16), sdesc_128(k + at, 16), idesc_s, i > 0);
-                }
-                mma_commit(&s_full[s]);
-            };
-            auto output = [&](int s, uint32_t tile) { // O_s += P_s V
-                const uint32_t v = smem_u32(vs + (tile % NS) * S::kKV);
-#pragma unroll
-                for (int i = 0; i < kTile / 16; ++i) {
-                    mma_f16_ta(tmem + kColO + s * kTile, tmem + s * kTile + i * 8, sdesc_128(v + i * 2048, S::kSlab),
-                               idesc_o);
-                }
-                mma_commit(&o_done[s]);
-            };
             items([&](int, const Request&, int64_t, int, int, int t0, int t1) {
-                const int nt = t1 - t0;
-                bool ok = wait(&q_full, q_uses & 1);
-                ++q_uses;
-                // first scores of both groups
+                bool ok = wait(&q_full, items_done & 1);
+                ++items_done;
+                const uint32_t first = uses;
+                for (int i = kTiles == 2 ? 0 : s; i < t1 - t0; i += kTiles == 2 ? 1 : 2, ++uses) {
+                    const uint32_t st = (n + i) % NS, phase = ((n + i) / NS) & 1;
+                    // S = Q K^T, where the last product has read the weights
+                    ok = ok && wait(&k_full[st], phase);
+                    ok = ok && (uses == first || wait(&o_done[s], (uses - 1) & 1));
+                    if (ok) {
+                        const uint32_t k = smem_u32(ks + st * S::kKV);
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const int i = kTiles == 2 ? 0 : s;
-                    if (i < nt) {
-                        ok = ok && wait(&k_full[(n + i) % NS], ((n + i) / NS) & 1);
-                        if (ok) {
-                            scores(s, n + i);
-                            if (kTiles == 1 || s == 1) {
-                                mma_commit(&k_empty[(n + i) % NS]);
-                            }
+                        for (int c = 0; c < DP / 16; ++c) {
+                            const uint32_t at = (c / 4) * S::kSlab + (c % 4) * 32;
+                            mma_f16(t_s, sdesc_128(q + at, 16), sdesc_128(k + at, 16), idesc_s, c > 0);
                         }
+                        mma_commit(&s_full[s]);
+                        mma_commit(&k_empty[st]);
+                    }
+                    // O += P V
+                    ok = ok && wait(&v_full[st], phase);
+                    ok = ok && wait(&p_full[s], uses & 1);
+                    if (ok) {
+                        const uint32_t v = smem_u32(vs + st * S::kKV);
+#pragma unroll
+                        for (int c = 0; c < kTile / 16; ++c) {
+                            mma_f16_ta(t_o, t_s + c * 8, sdesc_128(v + c * 2048, S::kSlab), idesc_o);
+                        }
+                        mma_commit(&o_done[s]);
+                        mma_commit(&v_empty[st]);
                     }
                 }
-                for (int i = 0; i < nt; ++i) {
-                    const uint32_t tile = n + i;
-                    ok = ok && wait(&v_full[tile % NS], (tile / NS) & 1);
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        if (kTiles == 1 && s != (i & 1)) {
-                            continue;
-                        }
-                        ok = ok && wait(&p_full[s], p_uses[s] & 1);
-                        if (ok) {
-                            output(s, tile);
-                            if (kTiles == 1 || s == 1) {
-                                mma_commit(&v_empty[tile % NS]);
-                            }
-                        }
-                        const int next = i + (kTiles == 2 ? 1 : 2);
-                        if (next < nt) {
-                            // the scores go where the weights that this product reads lie
-                            ok = ok && wait(&k_full[(n + next) % NS], ((n + next) / NS) & 1);
-                            ok = ok && wait(&o_done[s], p_uses[s] & 1);
-                            if (ok) {
-                                scores(s, n + next);
-                                if (kTiles == 1 || s == 1) {
-                                    mma_commit(&k_empty[(n + next) % NS]);
-                                }
-                            }
-                        }
-                        ++p_uses[s];
-                    }
-                }
-                n += nt;
+                n += t1 - t0;
             });
             // what was issued completes before tensor memory is freed
             mma_commit(&drain);
@@ -395,6 +382,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         __syncwarp();
     } else {
+        regs_up<208>();
         // ---- softmax: group s, one row a thread
         const int s = warp >> 2, wt = tid & 127;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -416,6 +404,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int row = (kTiles == 2 ? s * kTile : 0) + wt;
             const int tok = row < rows ? (rb * RT + row) / group : -1;
             const uint32_t* mask = a.mask != nullptr ? a.mask + (rq.first + max(tok, 0)) * g.mask_words : nullptr;
+            // What runs once an item is kept small (rolled loops): unrolled, its instructions came from L2 each time and an item
+            // cost as much as nine tiles.
             // the 16-byte chunks of the item's rows, in q and in out, shared by the 256 threads
             constexpr int kRowChunks = DP / 8, kRowStep = kSoftmax / kRowChunks, kRowSteps = RT / kRowStep;
             auto for_rows = [&](auto&& f) {
@@ -423,10 +413,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 int qr = tid / kRowChunks;
                 int qt = (rb * RT + qr) / group, hq = rb * RT + qr - qt * group;
                 const int dt = kRowStep / group, dh = kRowStep - dt * group;
-#pragma unroll
+#pragma unroll 1
                 for (int u = 0; u < kRowSteps; ++u) {
                     const int64_t t = rq.first + qt, h = static_cast<int64_t>(kvh) * group + hq;
-                    f(u, qr, ch, static_cast<const T*>(a.q) + t * g.q_stride + h * g.q_head_stride + ch * 8,
+                    f(qr, ch, static_cast<const T*>(a.q) + t * g.q_stride + h * g.q_head_stride + ch * 8,
                       static_cast<T*>(a.out) + t * g.o_stride + h * g.o_head_stride + ch * 8);
                     qr += kRowStep;
                     qt += dt;
@@ -437,24 +427,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                 }
             };
-            uint4 q_buf[kRowSteps];
             // ---- Q into shared memory (K-major slabs of 64), zero past the rows and head_dim
-            for_rows([&](int u, int qr, int ch, const T* src, T*) {
-                q_buf[u] = make_uint4(0, 0, 0, 0);
-                if (qr < rows && ch * 8 < g.head_dim) {
-                    q_buf[u] = *reinterpret_cast<const uint4*>(src);
-                }
+            for_rows([&](int qr, int ch, const T* src, T*) {
+                const bool in = qr < rows && ch * 8 < g.head_dim;
+                const int lr = qr % kTile, to = (qr / kTile) * S::kKV + (ch / 8) * S::kSlab + lr * 128 +
+                                                (((ch & 7) ^ (lr & 7)) << 4);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(qs + to)),
+                             "l"(in ? src : static_cast<const T*>(a.q)), "r"(in ? 16 : 0)
+                             : "memory");
             });
-#pragma unroll
-            for (int u = 0; u < kRowSteps; ++u) {
-                const int qr = tid / kRowChunks + u * kRowStep, ch = tid % kRowChunks, lr = qr % kTile;
-                uint4 x = q_buf[u];
-                if (flip) {
-                    x.x ^= 0x80008000u, x.y ^= 0x80008000u, x.z ^= 0x80008000u, x.w ^= 0x80008000u;
-                }
-                *reinterpret_cast<uint4*>(qs + (qr / kTile) * S::kKV + (ch / 8) * S::kSlab + lr * 128 +
-                                          (((ch & 7) ^ (lr & 7)) << 4)) = x;
-            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
             // places of this CTA's tiles without a block: then every tile looks its places up
             bool hole = false;
             for (int j = t0 * kTile / size + tid; j * static_cast<int64_t>(size) < min(rq.total, t1 * kTile); j += kSoftmax) {
@@ -464,23 +446,74 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 hole_word = 1;
                 bad = true;
             }
-            fence_proxy_async_smem();
-            mbar_arrive(&q_full);
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < DP; c += 32) {
                 tmem_st32(t_o + c, zeros);
             }
             tmem_wait_st();
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            if (flip) { // a thread's own chunks
+                for_rows([&](int qr, int ch, const T*, T*) {
+                    const int lr = qr % kTile;
+                    uint4* x = reinterpret_cast<uint4*>(qs + (qr / kTile) * S::kKV + (ch / 8) * S::kSlab + lr * 128 +
+                                                        (((ch & 7) ^ (lr & 7)) << 4));
+                    *x = make_uint4(x->x ^ 0x80008000u, x->y ^ 0x80008000u, x->z ^ 0x80008000u, x->w ^ 0x80008000u);
+                });
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&q_full);
             bar_named(1, kSoftmax);
             const bool holes = *const_cast<volatile int*>(&hole_word) != 0;
 
             float m = -INFINITY, z = 0.0f; // reference and sum of this row
+            // The reference for a tile whose largest score is `raw`: O and the sum move to a new one where it is too far
+            // below. O is at rest: the tile's scores were made after the last product.
+            auto refer = [&](float raw) {
+                const float now = raw == -INFINITY ? -INFINITY : raw * scale2;
+                if (!__any_sync(0xffffffffu, now > m + 8.0f)) {
+                    return;
+                }
+                const float to = fmaxf(m, now), keep = to == -INFINITY ? 1.0f : exp2_fast(m - to);
+                if (__any_sync(0xffffffffu, m > -INFINITY)) {
+#pragma unroll 1
+                    for (int c = 0; c < DP; c += 16) {
+                        float v[16];
+                        tmem_ld16(t_o + c, v);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            v[i] *= keep;
+                        }
+                        tmem_st16(t_o + c, v);
+                    }
+                    tmem_wait_st();
+                }
+                z *= keep;
+                m = to;
+            };
+            // The groups take turns at the exponentials: left alone they fall into step, both at them and then both
+            // waiting for their products (a tile of 256 rows 4,900 clocks, in turns MEASURED). Turns go by tile, group 0 first where both
+            // have it.
+            auto my_turn = [&](int t) {
+                if (kTiles == 2 ? s == 1 || t > t0 : t > t0) {
+                    bar_named(4 + s, kSoftmax);
+                }
+            };
+            auto pass_turn = [&](int t) {
+                if ((kTiles == 2 && s == 0) || t + 1 < t1) {
+                    bar_arrive(5 - s, kSoftmax);
+                }
+            };
+            auto at_rest = [&] { return m == -INFINITY ? 0.0f : m; };
             bool ok = !*abort_flag;
             for (int t = t0 + (kTiles == 2 ? 0 : s); t < t1; t += kTiles == 2 ? 1 : 2) {
                 const uint32_t tile = n + (t - t0);
                 const int j0 = t * kTile;
                 const bool plain = j0 + kTile <= old && !holes;
-                uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+                // bits of the places 32 w .. 32 w + 31 of the tile that this row's token sees
+                auto seen = [&](int w) {
+                    return tok < 0 ? 0u
+                                   : valid_of[s_uses & 1][s][w] & see_bits(mask, g.mask_words, tok, j0 + 32 * w - old);
+                };
                 const int mine = kTiles == 2 ? 0 : s; // whose odd[] the tile uses
                 if (!plain) {
                     // ---- V's rows that may not be multiplied: no such place, or not finite
@@ -493,7 +526,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                     const uint32_t valid = __ballot_sync(0xffffffffu, there);
                     ok = mbar_wait(&v_full[tile % NS], (tile / NS) & 1, abort_flag, a.err, args.bound) && ok;
-#pragma unroll
+#pragma unroll 1
                     for (int sl = 0; sl < S::kSlabs; ++sl) {
                         if (kTiles == 2 && S::kSlabs == 2 && sl != s) {
                             continue; // the groups share the slabs
@@ -503,7 +536,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
                         uint8_t* vr = vt + sl * S::kSlab + wt * 128;
                         bool odd_here = false;
-#pragma unroll
+#pragma unroll 2
                         for (int c = 0; c < 8; ++c) {
                             const uint4 x = *reinterpret_cast<const uint4*>(vr + ((c ^ (wt & 7)) << 4)); // no bank twice
 #pragma unroll
@@ -514,7 +547,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             }
                         }
                         if (!there || odd_here) {
-#pragma unroll
+#pragma unroll 1
                             for (int c = 0; c < 8; ++c) {
                                 *reinterpret_cast<uint4*>(vr + ((c ^ (wt & 7)) << 4)) = make_uint4(0, 0, 0, 0);
                             }
@@ -529,102 +562,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         valid_of[s_uses & 1][s][warp & 3] = valid;
                     }
                     bar_named(kTiles == 2 ? 1 : 2 + s, share);
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        see[w] = tok < 0 ? 0u
-                                         : valid_of[s_uses & 1][s][w] &
-                                               see_bits(mask, g.mask_words, tok, j0 + 32 * w - old);
-                    }
                 }
                 // ---- the row's scores
                 ok = mbar_wait(&s_full[s], s_uses & 1, abort_flag, a.err, args.bound) && ok;
                 __syncwarp();
                 tc_fence_after();
-                auto chunk = [&](int c, float (&x)[32]) {
-                    uint32_t v[32];
-                    tmem_ld32(t_s + c * 32, v);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        x[i] = __uint_as_float(v[i]);
-                    }
-                    if (!plain) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            x[i] = (see[c] >> i) & 1u ? x[i] : -INFINITY;
-                        }
-                    }
-                };
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float x[32];
-                    chunk(c, x);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        top[i & 3] = fmaxf(top[i & 3], x[i]);
-                    }
-                }
-                // -inf stays -inf whatever the scale (0 * -inf would not)
-                const float raw = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                const float now = raw == -INFINITY ? -INFINITY : raw * scale2;
-                if (__any_sync(0xffffffffu, now > m + 8.0f)) {
-                    const float to = fmaxf(m, now), keep = to == -INFINITY ? 1.0f : exp2_fast(m - to);
-                    if (__any_sync(0xffffffffu, m > -INFINITY)) { // O is at rest: this tile's scores were made after it
-                        for (int c = 0; c < DP; c += 32) {
-                            uint32_t v[32];
-                            tmem_ld32(t_o + c, v);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                v[i] = __float_as_uint(__uint_as_float(v[i]) * keep);
-                            }
-                            tmem_st32(t_o + c, v);
-                        }
-                        tmem_wait_st();
-                    }
-                    z *= keep;
-                    m = to;
-                }
-                const float ref = m == -INFINITY ? 0.0f : m;
-                if (!plain) {
-                    // ---- places whose values are not finite, for the rows that see them
-#pragma unroll 1
-                    for (int sw = 0; sw < S::kSlabs * 4; ++sw) {
-                        const int sl = sw >> 2, w = sw & 3;
-                        for (uint32_t left = odd[s_uses & 1][mine][sl][w]; left != 0; left &= left - 1) {
-                            const int key = w * 32 + __ffs(left) - 1, j = j0 + key;
-                            uint32_t raw_s;
-                            tmem_ld1(t_s + key, raw_s);
-                            tmem_wait_ld();
-                            const bool sees = (see[0] >> (key & 31) & 1u & (w == 0)) | (see[1] >> (key & 31) & 1u & (w == 1)) |
-                                              (see[2] >> (key & 31) & 1u & (w == 2)) | (see[3] >> (key & 31) & 1u & (w == 3));
-                            const float p = sees ? exp2_fast(fmaf(__uint_as_float(raw_s), scale2, -ref)) : 0.0f;
-                            const int64_t b = table[j / size];
-                            const T* v = static_cast<const T*>(a.vc) + b * g.vc_block_stride + (j % size) * g.vc_place_stride +
-                                         kvh * g.vc_head_stride + sl * 64;
-                            for (int c = 0; c < 64; c += 32) {
-                                uint32_t o[32];
-                                tmem_ld32(t_o + sl * 64 + c, o);
-                                tmem_wait_ld();
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) {
-                                    const bool in = sl * 64 + c + i < g.head_dim;
-                                    const float f = in ? to_f32(v[in ? c + i : 0]) : 0.0f;
-                                    o[i] = p > 0.0f ? __float_as_uint(__uint_as_float(o[i]) + p * f) : o[i];
-                                }
-                                tmem_st32(t_o + sl * 64 + c, o);
-                                tmem_wait_st();
-                            }
-                        }
-                    }
-                }
-                // ---- weights, packed over the scores; their sum keeps all bits
                 float zz[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float x[32];
-                    chunk(c, x);
+                // 32 scores to weights, packed over the scores; their sum keeps all bits
+                auto weights = [&](int c, const float* x, float ref) {
                     uint32_t pk[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
@@ -635,7 +580,88 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         pk[i] = pack2<T>(p0, p1);
                     }
                     tmem_st16u(t_s + c * 16, pk);
+                };
+                if (plain) { // the row stays in registers
+                    float x[kTile];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t v[32];
+                        tmem_ld32(t_s + c * 32, v);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            x[c * 32 + i] = __uint_as_float(v[i]);
+                        }
+                    }
+                    float top[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                    for (int i = 4; i < kTile; ++i) {
+                        top[i & 3] = fmaxf(top[i & 3], x[i]);
+                    }
+                    refer(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+                    const float ref = at_rest();
+                    my_turn(t);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        weights(c, x + c * 32, ref);
+                    }
+                } else {
+                    auto chunk = [&](int c, float (&x)[32]) {
+                        const uint32_t see = seen(c);
+                        uint32_t v[32];
+                        tmem_ld32(t_s + c * 32, v);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            x[i] = (see >> i) & 1u ? __uint_as_float(v[i]) : -INFINITY;
+                        }
+                    };
+                    float top = -INFINITY;
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        float x[32];
+                        chunk(c, x);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            top = fmaxf(top, x[i]);
+                        }
+                    }
+                    refer(top);
+                    // ---- places whose values are not finite, for the rows that see them
+#pragma unroll 1
+                    for (int sw = 0; sw < S::kSlabs * 4; ++sw) {
+                        const int sl = sw >> 2, w = sw & 3;
+                        for (uint32_t left = odd[s_uses & 1][mine][sl][w]; left != 0; left &= left - 1) {
+                            const int key = w * 32 + __ffs(left) - 1, j = j0 + key;
+                            uint32_t raw_s;
+                            tmem_ld1(t_s + key, raw_s);
+                            const bool sees = (seen(w) >> (key & 31)) & 1u;
+                            const float p = sees ? exp2_fast(fmaf(__uint_as_float(raw_s), scale2, -at_rest())) : 0.0f;
+                            const int64_t b = table[j / size];
+                            const T* v = static_cast<const T*>(a.vc) + b * g.vc_block_stride + (j % size) * g.vc_place_stride +
+                                         kvh * g.vc_head_stride + sl * 64;
+#pragma unroll 1
+                            for (int c = 0; c < 64; c += 16) {
+                                float o[16];
+                                tmem_ld16(t_o + sl * 64 + c, o);
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) {
+                                    const bool in = p > 0.0f && sl * 64 + c + i < g.head_dim;
+                                    o[i] += in ? p * to_f32(v[in ? c + i : 0]) : 0.0f;
+                                }
+                                tmem_st16(t_o + sl * 64 + c, o);
+                                tmem_wait_st();
+                            }
+                        }
+                    }
+                    const float ref = at_rest();
+                    my_turn(t);
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        float x[32];
+                        chunk(c, x);
+                        weights(c, x, ref);
+                    }
                 }
+                pass_turn(t);
                 z += (zz[0] + zz[1]) + (zz[2] + zz[3]);
                 tmem_wait_st();
                 tc_fence_before();
@@ -698,7 +724,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             auto finish = [&](float top, float sum) { // after stage() of all elements
                 bar_named(1, kSoftmax);
                 if (clean) {
-                    for_rows([&](int, int qr, int ch, const T*, T* dst) {
+                    for_rows([&](int qr, int ch, const T*, T* dst) {
                         if (qr < rows && ch * 8 < g.head_dim) {
                             *reinterpret_cast<uint4*>(dst) =
                                 *reinterpret_cast<const uint4*>(qs + qr * DP * 2 + ((ch ^ (qr & 7)) << 4));
@@ -718,14 +744,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 float x[32];
                 __syncwarp();
                 tmem_ld32(t_o + c0 + c, v);
-                tmem_wait_ld();
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
                     x[i] = __uint_as_float(v[i]);
                 }
                 if (kTiles == 1) {
                     tmem_ld32(tmem + lanes + kColO + (1 - s) * kTile + c0 + c, v);
-                    tmem_wait_ld();
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         const float p = ff != 0.0f ? ff * x[i] : 0.0f;
@@ -772,18 +796,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
                         top = -INFINITY;
                         sum = 0.0f;
+                        float y[32], y_next[32];
+                        float2 ml, ml_next;
+                        auto piece_of = [&](int p, float (&o)[32], float2& e) {
+                            const int64_t at = 2 * static_cast<int64_t>(p) + (p == p0 ? 1 : 0);
+                            const float* src = args.part_o + (at * DP + c0 + c) * RT + row;
+                            e = live ? __ldcg(args.part_ml + at * RT + row) : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                o[i] = live ? __ldcg(src + i * RT) : 0.0f;
+                            }
+                        };
+                        piece_of(p0, y, ml);
 #pragma unroll 1
                         for (int p = p0; p <= p1; ++p) {
-                            const int64_t at = 2 * static_cast<int64_t>(p) + (p == p0 ? 1 : 0);
-                            const float* o = args.part_o + at * DP * RT + row;
-                            float y[32];
-                            float2 ml = make_float2(-INFINITY, 0.0f);
-                            if (live) {
-                                ml = __ldcg(args.part_ml + at * RT + row);
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) {
-                                    y[i] = __ldcg(o + static_cast<int64_t>(c0 + c + i) * RT);
-                                }
+                            if (p < p1) { // in flight while this one is added
+                                piece_of(p + 1, y_next, ml_next);
                             }
                             const float to = fmaxf(top, ml.x), ref = to == -INFINITY ? 0.0f : to;
                             const float f = exp2_fast(top - ref), h = exp2_fast(ml.x - ref);
@@ -791,9 +819,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             sum = f * sum + h * ml.y;
 #pragma unroll
                             for (int i = 0; i < 32; ++i) {
-                                // a piece that saw nothing adds nothing
-                                x[i] = live && h != 0.0f ? f * x[i] + h * y[i] : f * x[i];
+                                x[i] = h != 0.0f ? f * x[i] + h * y[i] : f * x[i]; // a piece that saw nothing adds nothing
+                                y[i] = y_next[i];
                             }
+                            ml = ml_next;
                         }
                         stage(c0 + c, x, sum);
                     }
