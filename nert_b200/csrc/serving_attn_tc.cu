@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 int qr = tid / kRowChunks;
                 int qt = (rb * RT + qr) / group, hq = rb * RT + qr - qt * group;
                 const int dt = kRowStep / group, dh = kRowStep - dt * group;
-#pragma unroll 1
+#pragma unroll 4
                 for (int u = 0; u < kRowSteps; ++u) {
                     const int64_t t = rq.first + qt, h = static_cast<int64_t>(kvh) * group + hq;
                     f(qr, ch, static_cast<const T*>(a.q) + t * g.q_stride + h * g.q_head_stride + ch * 8,
@@ -509,10 +509,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const uint32_t tile = n + (t - t0);
                 const int j0 = t * kTile;
                 const bool plain = j0 + kTile <= old && !holes;
-                // bits of the places 32 w .. 32 w + 31 of the tile that this row's token sees
-                auto seen = [&](int w) {
-                    return tok < 0 ? 0u
-                                   : valid_of[s_uses & 1][s][w] & see_bits(mask, g.mask_words, tok, j0 + 32 * w - old);
+                // bits of the tile's places that this row's token sees, if they are there
+                uint32_t sees[4] = {0, 0, 0, 0};
+                auto seen = [&](int w) { // of places 32 w .. 32 w + 31
+                    return (w == 0 ? sees[0] : w == 1 ? sees[1] : w == 2 ? sees[2] : sees[3]) & valid_of[s_uses & 1][s][w];
                 };
                 const int mine = kTiles == 2 ? 0 : s; // whose odd[] the tile uses
                 if (!plain) {
@@ -525,6 +525,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         there = b >= 0 && b < g.num_blocks;
                     }
                     const uint32_t valid = __ballot_sync(0xffffffffu, there);
+                    if (tok >= 0) {
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            sees[w] = see_bits(mask, g.mask_words, tok, j0 + 32 * w - old);
+                        }
+                    }
                     ok = mbar_wait(&v_full[tile % NS], (tile / NS) & 1, abort_flag, a.err, args.bound) && ok;
 #pragma unroll 1
                     for (int sl = 0; sl < S::kSlabs; ++sl) {
@@ -633,8 +639,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             const int key = w * 32 + __ffs(left) - 1, j = j0 + key;
                             uint32_t raw_s;
                             tmem_ld1(t_s + key, raw_s);
-                            const bool sees = (seen(w) >> (key & 31)) & 1u;
-                            const float p = sees ? exp2_fast(fmaf(__uint_as_float(raw_s), scale2, -at_rest())) : 0.0f;
+                                                        const float p = (seen(w) >> (key & 31)) & 1u ? exp2_fast(fmaf(__uint_as_float(raw_s), scale2, -at_rest())) : 0.0f;
                             const int64_t b = table[j / size];
                             const T* v = static_cast<const T*>(a.vc) + b * g.vc_block_stride + (j % size) * g.vc_place_stride +
                                          kvh * g.vc_head_stride + sl * 64;
@@ -707,7 +712,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int c0 = kTiles == 2 ? 0 : s * kCols;
             // finished values of a row's 32 elements from d on, through Q's shared memory (its products are
             // done) so that the stores to out are of whole rows: a row a thread, each store met 32 lines
-            auto stage = [&](int d, const float (&x)[32], float sum) {
+            auto stage = [&](int d, const float* x, float sum) {
                 const float inv = 1.0f / sum;
                 const bool none = sum == 0.0f; // no place was seen
 #pragma unroll
@@ -736,8 +741,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                 }
             };
-            // a piece lies in its slot element by element, the rows together
-            float* piece = args.part_o + slot * DP * RT + row;
+            // a piece lies in its slot four elements by four, the rows together
+            float4* piece = reinterpret_cast<float4*>(args.part_o) + slot * (DP / 4) * RT + row;
 #pragma unroll 1
             for (int c = 0; c < kCols; c += 32) {
                 uint32_t v[32];
@@ -761,8 +766,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     stage(c0 + c, x, zs);
                 } else if (live) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        __stcg(piece + static_cast<int64_t>(c0 + c + i) * RT, x[i]);
+                    for (int i = 0; i < 32; i += 4) {
+                        __stcg(piece + (c0 + c + i) / 4 * RT, make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]));
                     }
                 }
             }
@@ -787,44 +792,43 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     // all pieces are there: added in the order of their CTAs
                     __threadfence();
                     float top = -INFINITY, sum = 0.0f;
+                    constexpr int kJoin = kCols < 64 ? kCols : 64; // elements of a row at a time
 #pragma unroll 1
-                    for (int c = 0; c < kCols; c += 32) {
-                        float x[32];
+                    for (int c = 0; c < kCols; c += kJoin) {
+                        float x[kJoin];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
+                        for (int i = 0; i < kJoin; ++i) {
                             x[i] = 0.0f;
                         }
                         top = -INFINITY;
                         sum = 0.0f;
-                        float y[32], y_next[32];
-                        float2 ml, ml_next;
-                        auto piece_of = [&](int p, float (&o)[32], float2& e) {
-                            const int64_t at = 2 * static_cast<int64_t>(p) + (p == p0 ? 1 : 0);
-                            const float* src = args.part_o + (at * DP + c0 + c) * RT + row;
-                            e = live ? __ldcg(args.part_ml + at * RT + row) : make_float2(-INFINITY, 0.0f);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                o[i] = live ? __ldcg(src + i * RT) : 0.0f;
-                            }
-                        };
-                        piece_of(p0, y, ml);
 #pragma unroll 1
                         for (int p = p0; p <= p1; ++p) {
-                            if (p < p1) { // in flight while this one is added
-                                piece_of(p + 1, y_next, ml_next);
+                            const int64_t at = 2 * static_cast<int64_t>(p) + (p == p0 ? 1 : 0);
+                            const float4* src = reinterpret_cast<const float4*>(args.part_o) + (at * DP + c0 + c) / 4 * RT + row;
+                            const float2 ml = live ? __ldcg(args.part_ml + at * RT + row) : make_float2(-INFINITY, 0.0f);
+                            float4 y[kJoin / 4];
+#pragma unroll
+                            for (int i = 0; i < kJoin / 4; ++i) {
+                                y[i] = live ? __ldcg(src + i * RT) : make_float4(0, 0, 0, 0);
                             }
                             const float to = fmaxf(top, ml.x), ref = to == -INFINITY ? 0.0f : to;
                             const float f = exp2_fast(top - ref), h = exp2_fast(ml.x - ref);
                             top = to;
                             sum = f * sum + h * ml.y;
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                x[i] = h != 0.0f ? f * x[i] + h * y[i] : f * x[i]; // a piece that saw nothing adds nothing
-                                y[i] = y_next[i];
+                            for (int i = 0; i < kJoin / 4; ++i) {
+                                const float* z4 = &y[i].x;
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) { // a piece that saw nothing adds nothing
+                                    x[4 * i + k] = h != 0.0f ? f * x[4 * i + k] + h * z4[k] : f * x[4 * i + k];
+                                }
                             }
-                            ml = ml_next;
                         }
-                        stage(c0 + c, x, sum);
+#pragma unroll
+                        for (int i = 0; i < kJoin; i += 32) {
+                            stage(c0 + c + i, x + i, sum);
+                        }
                     }
                     finish(top, sum);
                 }
