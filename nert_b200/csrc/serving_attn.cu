@@ -109,8 +109,9 @@ struct Shape {
 };
 
 template <typename T, int DP, int WR, int WK>
-__global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(TreeAttnArgs a, int group, float* part_o,
-                                                                 float2* part_ml, uint32_t* tickets) {
+__global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(const __grid_constant__ TreeAttnArgs a, int group,
+                                                                 int sms, float* part_o, float2* part_ml,
+                                                                 uint32_t* tickets) {
     using S = Shape<T, DP, WR, WK>;
     constexpr int NT = S::kThreads, RT = S::RT, KT = S::KT, KW = S::KW, NS = S::NS;
     constexpr int NB = KW / 8; // 8-place column blocks of a warp's scores
@@ -134,7 +135,7 @@ __global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(TreeAttnArgs a,
     const float scale2 = g.scale * kLog2e;
     bool bad = false;
 
-    const Span span = find_span<RT, KT, NT>(a, group, red, found, bad);
+    const Span span = find_span<RT, KT, NT>(a, group, sms, red, found, bad);
     spare_tokens<T>(a, tid, NT);
     const int64_t W = span.W, grid = span.grid, w1 = span.w1;
     int r = span.request;
@@ -150,7 +151,7 @@ __global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(TreeAttnArgs a,
         }
         // ---- the item and this CTA's tiles of it
         const int64_t item = (w - r_unit) / rq.per_item();
-        const int64_t item_w0 = r_unit + item * rq.per_item() + Request::kExtra, item_w1 = item_w0 + rq.tiles;
+        const int64_t item_w0 = r_unit + item * rq.per_item() + rq.extra, item_w1 = item_w0 + rq.tiles;
         const int64_t from = max(w, item_w0);
         w = min(w1, item_w1);
         if (from >= w) {
@@ -609,7 +610,7 @@ void launch_attn(nb2_device* dev, const TreeAttnArgs& a) {
     const int grid = dev->num_sms * per_sm[dev->ordinal];
     const size_t o_bytes = static_cast<size_t>(grid) * 2 * S::RT * DP * 4;
     uint8_t* ws = static_cast<uint8_t*>(dev->scratch(o_bytes + static_cast<size_t>(grid) * 2 * S::RT * 8));
-    kernel<<<grid, S::kThreads, S::kSmem, dev->stream>>>(a, static_cast<int>(a.g.q_heads / a.g.kv_heads),
+    kernel<<<grid, S::kThreads, S::kSmem, dev->stream>>>(a, static_cast<int>(a.g.q_heads / a.g.kv_heads), dev->num_sms,
                                                          reinterpret_cast<float*>(ws),
                                                          reinterpret_cast<float2*>(ws + o_bytes), dev->tickets(grid));
     check_cuda(cudaGetLastError(), "tree attention launch");

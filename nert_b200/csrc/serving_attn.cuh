@@ -17,9 +17,8 @@ struct Request {
     int row_blocks; // blocks of its n * group rows
     int tiles;      // tiles of its places, at least one so that rows without places are written
     bool bad;
-    // What beginning and ending an item costs a CTA, in tiles: Q, the pipeline's fill, the stores and the join.
-    static constexpr int kExtra = 2;
-    __device__ __forceinline__ int per_item() const { return tiles + kExtra; }
+    int extra;      // what beginning and ending an item costs a CTA, in tiles: Q, the pipeline's fill, the stores
+    __device__ __forceinline__ int per_item() const { return tiles + extra; }
     __device__ __forceinline__ int64_t units(int64_t kv_heads) const {
         return static_cast<int64_t>(row_blocks) * kv_heads * per_item();
     }
@@ -43,6 +42,7 @@ __device__ __forceinline__ Request request_at(const TreeAttnArgs& a, int r, int 
     q.total = q.bad ? 0 : static_cast<int>(total);
     q.row_blocks = static_cast<int>((static_cast<int64_t>(q.n) * group + RT - 1) / RT);
     q.tiles = max(1, (q.total + KT - 1) / KT);
+    q.extra = KT == 128 ? 5 : 2; // measured: fewer or more are slower by 5% on mixed lengths
     return q;
 }
 
@@ -98,57 +98,70 @@ __device__ __forceinline__ void store_row4(const TreeAttnArgs& a, int64_t first,
 }
 
 // The pieces of an item in the slots of CTAs c0 .. c1 (the first left its piece in its second slot,
-// the others theirs in their first), added in that order and stored; NT threads.
-template <typename T, int DP, int RT, int NT>
-__device__ __forceinline__ void join_pieces(const TreeAttnArgs& a, const float* part_o, const float2* part_ml, int c0, int c1,
-                                            int64_t first, int64_t kvh, int group, int rho0, int rows, int tid) {
-    // kAhead elements of a thread at a time: one after another, the loads of a piece took longer than its tiles
-    constexpr int kAhead = 8;
-    for (int i0 = tid; i0 < rows * (DP / 4); i0 += kAhead * NT) {
-        float m[kAhead], z[kAhead];
-        float4 x[kAhead];
+// the others theirs in their first), added in that order and stored; NT threads. A thread takes kElems groups of
+// four elements through kPieces pieces at a time, all their loads in flight: one after another the loads of a short
+// item's pieces (up to one a tile) took longer than its tiles.
+template <typename T, int DP, int RT, int NT, int kElems, int kPieces>
+__device__ __forceinline__ void join_pieces_as(const TreeAttnArgs& a, const float* part_o, const float2* part_ml, int c0,
+                                               int c1, int64_t first, int64_t kvh, int group, int rho0, int rows, int tid) {
+    for (int i0 = tid; i0 < rows * (DP / 4); i0 += kElems * NT) {
+        float m[kElems], z[kElems];
+        float4 x[kElems];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
+        for (int u = 0; u < kElems; ++u) {
             m[u] = -INFINITY;
             z[u] = 0.0f;
             x[u] = make_float4(0, 0, 0, 0);
         }
-        for (int c = c0; c <= c1; ++c) {
-            const int64_t slot = 2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0);
-            float2 ml[kAhead];
-            float4 y[kAhead];
+#pragma unroll 1
+        for (int c = c0; c <= c1; c += kPieces) {
+            float2 ml[kPieces][kElems];
+            float4 y[kPieces][kElems];
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int i = i0 + u * NT, row = i / (DP / 4), d = (i - row * (DP / 4)) * 4;
-                if (row < rows && d < a.g.head_dim) {
-                    ml[u] = __ldcg(&part_ml[slot * RT + row]);
-                    y[u] = __ldcg(reinterpret_cast<const float4*>(part_o + (slot * RT + row) * DP + d));
-                } else {
-                    ml[u] = make_float2(-INFINITY, 0.0f);
-                    y[u] = make_float4(0, 0, 0, 0);
+            for (int p = 0; p < kPieces; ++p) {
+                const int64_t slot = 2 * static_cast<int64_t>(c + p) + (c + p == c0 ? 1 : 0);
+#pragma unroll
+                for (int u = 0; u < kElems; ++u) {
+                    const int i = i0 + u * NT, row = i / (DP / 4), d = (i - row * (DP / 4)) * 4;
+                    ml[p][u] = make_float2(-INFINITY, 0.0f);
+                    if (c + p <= c1 && row < rows && d < a.g.head_dim) {
+                        ml[p][u] = __ldcg(&part_ml[slot * RT + row]);
+                        y[p][u] = __ldcg(reinterpret_cast<const float4*>(part_o + (slot * RT + row) * DP + d));
+                    }
                 }
             }
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const float to = fmaxf(m[u], ml[u].x), ref = to == -INFINITY ? 0.0f : to;
-                const float f = exp2_fast(m[u] - ref), h = exp2_fast(ml[u].x - ref);
-                m[u] = to;
-                z[u] = f * z[u] + h * ml[u].y;
-                if (h != 0.0f) { // a piece that saw nothing adds nothing
-                    x[u].x = f * x[u].x + h * y[u].x;
-                    x[u].y = f * x[u].y + h * y[u].y;
-                    x[u].z = f * x[u].z + h * y[u].z;
-                    x[u].w = f * x[u].w + h * y[u].w;
+            for (int p = 0; p < kPieces; ++p) {
+#pragma unroll
+                for (int u = 0; u < kElems; ++u) {
+                    const float to = fmaxf(m[u], ml[p][u].x), ref = to == -INFINITY ? 0.0f : to;
+                    const float f = exp2_fast(m[u] - ref), h = exp2_fast(ml[p][u].x - ref);
+                    m[u] = to;
+                    z[u] = f * z[u] + h * ml[p][u].y;
+                    x[u].x *= f, x[u].y *= f, x[u].z *= f, x[u].w *= f;
+                    if (h != 0.0f) { // a piece that saw nothing adds nothing
+                        x[u].x += h * y[p][u].x, x[u].y += h * y[p][u].y, x[u].z += h * y[p][u].z, x[u].w += h * y[p][u].w;
+                    }
                 }
             }
         }
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
+        for (int u = 0; u < kElems; ++u) {
             const int i = i0 + u * NT, row = i / (DP / 4), d = (i - row * (DP / 4)) * 4;
             if (row < rows && d < a.g.head_dim) {
                 store_row4<T>(a, first, kvh, group, rho0 + row, d, x[u], m[u], z[u]);
             }
         }
+    }
+}
+
+template <typename T, int DP, int RT, int NT>
+__device__ __forceinline__ void join_pieces(const TreeAttnArgs& a, const float* part_o, const float2* part_ml, int c0, int c1,
+                                            int64_t first, int64_t kvh, int group, int rho0, int rows, int tid) {
+    if (rows * (DP / 4) <= 2 * NT) {
+        join_pieces_as<T, DP, RT, NT, 1, 8>(a, part_o, part_ml, c0, c1, first, kvh, group, rho0, rows, tid);
+    } else {
+        join_pieces_as<T, DP, RT, NT, 4, 2>(a, part_o, part_ml, c0, c1, first, kvh, group, rho0, rows, tid);
     }
 }
 
@@ -180,8 +193,13 @@ struct Span {
     int64_t request_unit; // first unit of that request
 };
 
+// Spans shorter than kMinSpan units are not made while `least` CTAs have one: more CTAs an SM would then read no
+// faster, and each adds a piece to the join.
+constexpr int kMinSpan = 4;
+
 template <int RT, int KT, int NT>
-__device__ __forceinline__ Span find_span(const TreeAttnArgs& a, int group, int64_t* red, int64_t* found, bool& bad) {
+__device__ __forceinline__ Span find_span(const TreeAttnArgs& a, int group, int least, int64_t* red, int64_t* found,
+                                          bool& bad) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int B = static_cast<int>(a.g.batch);
     const int64_t cta = blockIdx.x;
@@ -194,7 +212,7 @@ __device__ __forceinline__ Span find_span(const TreeAttnArgs& a, int group, int6
         mine = r == tid ? s.W : mine;
     }
     s.W = block_sum<NT>(s.W, red);
-    s.grid = min(static_cast<int64_t>(gridDim.x), s.W); // no span is empty
+    s.grid = min(static_cast<int64_t>(gridDim.x), max(s.W / kMinSpan, min(s.W, static_cast<int64_t>(least)))); // no span is empty
     if (cta >= s.grid) {
         return s;
     }

@@ -35,6 +35,7 @@ namespace {
 constexpr int kTcThreads = 384; // two softmax groups; a TMA warp, two MMA warps and one that only makes up the third group
 constexpr int kSoftmax = 256; // threads of the two softmax groups
 constexpr int kTile = 128;    // places of a tile, rows of a block
+constexpr int kHalf = 64;     // places of a score product
 constexpr uint32_t kColO = 256;
 constexpr int kTcRows = 32; // rows a key/value head above which this kernel is taken
 
@@ -84,6 +85,25 @@ __device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t (&r)[32]) {
                    "=r"(r[30]), "=r"(r[31])
                  : "r"(t));
 }
+// 32 lanes x 64 columns to registers, complete.
+__device__ __forceinline__ void tmem_ld64(uint32_t t, uint32_t (&r)[64]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+                 "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,"
+                 "%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,"
+                 "%60,%61,%62,%63}, [%64];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+                   "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+                   "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+                   "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+                   "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+                 : "r"(t)
+                 : "memory");
+}
+
 __device__ __forceinline__ void tmem_ld1(uint32_t t, uint32_t& r) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;" : "=r"(r) : "r"(t) : "memory");
 }
@@ -129,10 +149,6 @@ static_assert((2 * 208 + 88) * 128 <= 168 * 384, "the groups share what the laun
 
 __device__ __forceinline__ void bar_named(int id, int threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-
-__device__ __forceinline__ void bar_arrive(int id, int threads) {
-    asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
 template <typename T>
@@ -197,7 +213,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tc_dyn) + 1023) & ~uintptr_t(1023));
     uint8_t* ks = qs + S::kQ;
     uint8_t* vs = ks + NS * S::kKV;
-    __shared__ uint64_t k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], s_full[2], p_full[2], o_done[2], q_full, drain;
+    __shared__ uint64_t k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], s_full[2][2], p_full[2][2], o_done[2], q_full,
+        drain;
     __shared__ int64_t red[kTcThreads / 32], found[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word, is_last, hole_word;
@@ -218,8 +235,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_init(&v_empty[i], kTiles);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], kTile);
+            for (int h = 0; h < 2; ++h) {
+                mbar_init(&s_full[i][h], 1);
+                mbar_init(&p_full[i][h], kTile);
+            }
             mbar_init(&o_done[i], 1);
         }
         mbar_init(&q_full, kSoftmax);
@@ -236,7 +255,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         prefetch_tmap(&k_map);
         prefetch_tmap(&v_map);
     }
-    const Span span = find_span<RT, kTile, kTcThreads>(a, group, red, found, bad);
+    const Span span = find_span<RT, kTile, kTcThreads>(a, group, gridDim.x, red, found, bad);
     spare_tokens<T>(a, tid, kTcThreads);
     tc_fence_before();
     __syncthreads();
@@ -257,7 +276,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 rq = request_at<RT, kTile>(a, ++r, group);
             }
             const int64_t item = (w - r_unit) / rq.per_item();
-            const int64_t item_w0 = r_unit + item * rq.per_item() + Request::kExtra; // its first tile
+            const int64_t item_w0 = r_unit + item * rq.per_item() + rq.extra; // its first tile
             const int64_t from = max(w, item_w0);
             w = min(span.w1, item_w0 + rq.tiles);
             if (from < w) {
@@ -332,7 +351,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // tensor cores idle while it looked for the next work (attention of 8 long contexts 236 us, with two threads MEASURED).
             const int s = warp - 9;
             uint32_t n = 0, items_done = 0, uses = 0; // tiles of all items so far, items, this group's tiles
-            const uint32_t idesc_s = idesc_f16(kBf16, kTile, false), idesc_o = idesc_f16(kBf16, DP, true);
+            const uint32_t idesc_s = idesc_f16(kBf16, kHalf, false), idesc_o = idesc_f16(kBf16, DP, true);
             const uint32_t q = smem_u32(qs + (kTiles == 2 ? s * S::kKV : 0)), t_s = tmem + s * kTile,
                            t_o = tmem + kColO + s * kTile;
             auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -343,33 +362,51 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             items([&](int, const Request&, int64_t, int, int, int t0, int t1) {
                 bool ok = wait(&q_full, items_done & 1);
                 ++items_done;
-                const uint32_t first = uses;
-                for (int i = kTiles == 2 ? 0 : s; i < t1 - t0; i += kTiles == 2 ? 1 : 2, ++uses) {
-                    const uint32_t st = (n + i) % NS, phase = ((n + i) / NS) & 1;
-                    // S = Q K^T, where the last product has read the weights
-                    ok = ok && wait(&k_full[st], phase);
-                    ok = ok && (uses == first || wait(&o_done[s], (uses - 1) & 1));
+                constexpr int kStep = kTiles == 2 ? 1 : 2;
+                const int i0 = kTiles == 2 ? 0 : s, nt = t1 - t0;
+                // S = Q K^T of half h of a tile; the last half's commit gives K back
+                auto scores = [&](int i, int h) {
+                    const uint32_t st = (n + i) % NS;
+                    ok = ok && wait(&k_full[st], ((n + i) / NS) & 1);
                     if (ok) {
-                        const uint32_t k = smem_u32(ks + st * S::kKV);
+                        const uint32_t k = smem_u32(ks + st * S::kKV) + h * kHalf * 128;
 #pragma unroll
                         for (int c = 0; c < DP / 16; ++c) {
                             const uint32_t at = (c / 4) * S::kSlab + (c % 4) * 32;
-                            mma_f16(t_s, sdesc_128(q + at, 16), sdesc_128(k + at, 16), idesc_s, c > 0);
+                            mma_f16(t_s + h * kHalf, sdesc_128(q + at, 16), sdesc_128(k + at, 16), idesc_s, c > 0);
                         }
-                        mma_commit(&s_full[s]);
-                        mma_commit(&k_empty[st]);
+                        mma_commit(&s_full[s][h]);
+                        if (h == 1) {
+                            mma_commit(&k_empty[st]);
+                        }
                     }
-                    // O += P V
-                    ok = ok && wait(&v_full[st], phase);
-                    ok = ok && wait(&p_full[s], uses & 1);
-                    if (ok) {
-                        const uint32_t v = smem_u32(vs + st * S::kKV);
+                };
+                if (i0 < nt) {
+                    scores(i0, 0);
+                    scores(i0, 1);
+                }
+                for (int i = i0; i < nt; i += kStep, ++uses) {
+                    const uint32_t st = (n + i) % NS;
+                    ok = ok && wait(&v_full[st], ((n + i) / NS) & 1);
 #pragma unroll
-                        for (int c = 0; c < kTile / 16; ++c) {
-                            mma_f16_ta(t_o, t_s + c * 8, sdesc_128(v + c * 2048, S::kSlab), idesc_o);
+                    for (int h = 0; h < 2; ++h) {
+                        // O += P V of the half, then the half's next scores where its weights were
+                        ok = ok && wait(&p_full[s][h], uses & 1);
+                        if (ok) {
+                            const uint32_t v = smem_u32(vs + st * S::kKV) + h * kHalf * 128;
+#pragma unroll
+                            for (int c = 0; c < kHalf / 16; ++c) {
+                                mma_f16_ta(t_o, t_s + h * kHalf + c * 8, sdesc_128(v + c * 2048, S::kSlab), idesc_o);
+                            }
+                            mma_commit(&o_done[s]);
+                            if (h == 1) {
+                                mma_commit(&v_empty[st]);
+                            }
                         }
-                        mma_commit(&o_done[s]);
-                        mma_commit(&v_empty[st]);
+                        if (i + kStep < nt) {
+                            ok = ok && wait(&o_done[s], h); // two products a tile: the first completes phase 0, the second 1
+                            scores(i + kStep, h);
+                        }
                     }
                 }
                 n += t1 - t0;
@@ -466,12 +503,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const bool holes = *const_cast<volatile int*>(&hole_word) != 0;
 
             float m = -INFINITY, z = 0.0f; // reference and sum of this row
-            // The reference for a tile whose largest score is `raw`: O and the sum move to a new one where it is too far
-            // below. O is at rest: the tile's scores were made after the last product.
+            bool ok = !*abort_flag;
+            uint32_t halves = 0; // of this item, whose weights this thread has given
+            // The reference for scores whose largest is `raw`: O and the sum move to a new one where it is too far below,
+            // after the last product.
             auto refer = [&](float raw) {
                 const float now = raw == -INFINITY ? -INFINITY : raw * scale2;
                 if (!__any_sync(0xffffffffu, now > m + 8.0f)) {
                     return;
+                }
+                if (halves > 0) {
+                    ok = mbar_wait(&o_done[s], (halves - 1) & 1, abort_flag, a.err, args.bound) && ok;
+                    __syncwarp();
+                    tc_fence_after();
                 }
                 const float to = fmaxf(m, now), keep = to == -INFINITY ? 1.0f : exp2_fast(m - to);
                 if (__any_sync(0xffffffffu, m > -INFINITY)) {
@@ -490,21 +534,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 z *= keep;
                 m = to;
             };
-            // The groups take turns at the exponentials: left alone they fall into step, both at them and then both
-            // waiting for their products (a tile of 256 rows 4,900 clocks, in turns MEASURED). Turns go by tile, group 0 first where both
-            // have it.
-            auto my_turn = [&](int t) {
-                if (kTiles == 2 ? s == 1 || t > t0 : t > t0) {
-                    bar_named(4 + s, kSoftmax);
-                }
-            };
-            auto pass_turn = [&](int t) {
-                if ((kTiles == 2 && s == 0) || t + 1 < t1) {
-                    bar_arrive(5 - s, kSoftmax);
-                }
-            };
             auto at_rest = [&] { return m == -INFINITY ? 0.0f : m; };
-            bool ok = !*abort_flag;
             for (int t = t0 + (kTiles == 2 ? 0 : s); t < t1; t += kTiles == 2 ? 1 : 2) {
                 const uint32_t tile = n + (t - t0);
                 const int j0 = t * kTile;
@@ -569,115 +599,120 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                     bar_named(kTiles == 2 ? 1 : 2 + s, share);
                 }
-                // ---- the row's scores
-                ok = mbar_wait(&s_full[s], s_uses & 1, abort_flag, a.err, args.bound) && ok;
-                __syncwarp();
-                tc_fence_after();
-                float zz[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                // 32 scores to weights, packed over the scores; their sum keeps all bits
-                auto weights = [&](int c, const float* x, float ref) {
-                    uint32_t pk[16];
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h, ++halves) {
+                    // ---- the row's scores of a half
+                    const uint32_t t_h = t_s + h * kHalf;
+                    ok = mbar_wait(&s_full[s][h], s_uses & 1, abort_flag, a.err, args.bound) && ok;
+                    __syncwarp();
+                    tc_fence_after();
+                    float zz[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    // 32 scores to weights, packed over the scores; their sum keeps all bits
+                    auto weights = [&](int c, const float* x, float ref) {
+                        uint32_t pk[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float p0 = exp2_fast(fmaf(x[2 * i], scale2, -ref));
-                        const float p1 = exp2_fast(fmaf(x[2 * i + 1], scale2, -ref));
-                        zz[(2 * i) & 3] += p0;
-                        zz[(2 * i + 1) & 3] += p1;
-                        pk[i] = pack2<T>(p0, p1);
-                    }
-                    tmem_st16u(t_s + c * 16, pk);
-                };
-                if (plain) { // the row stays in registers
-                    float x[kTile];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t v[32];
-                        tmem_ld32(t_s + c * 32, v);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            x[c * 32 + i] = __uint_as_float(v[i]);
+                        for (int i = 0; i < 16; ++i) {
+                            const float p0 = exp2_fast(fmaf(x[2 * i], scale2, -ref));
+                            const float p1 = exp2_fast(fmaf(x[2 * i + 1], scale2, -ref));
+                            zz[(2 * i) & 3] += p0;
+                            zz[(2 * i + 1) & 3] += p1;
+                            pk[i] = pack2<T>(p0, p1);
                         }
-                    }
-                    float top[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-                    for (int i = 4; i < kTile; ++i) {
-                        top[i & 3] = fmaxf(top[i & 3], x[i]);
-                    }
-                    refer(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
-                    const float ref = at_rest();
-                    my_turn(t);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        weights(c, x + c * 32, ref);
-                    }
-                } else {
-                    auto chunk = [&](int c, float (&x)[32]) {
-                        const uint32_t see = seen(c);
-                        uint32_t v[32];
-                        tmem_ld32(t_s + c * 32, v);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            x[i] = (see >> i) & 1u ? __uint_as_float(v[i]) : -INFINITY;
-                        }
+                        tmem_st16u(t_h + c * 16, pk);
                     };
-                    float top = -INFINITY;
-#pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        float x[32];
-                        chunk(c, x);
+                    if (plain) { // the row stays in registers
+                        float x[kHalf];
+                        uint32_t v[kHalf];
+                        tmem_ld64(t_h, v);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            top = fmaxf(top, x[i]);
+                        for (int i = 0; i < kHalf; ++i) {
+                            x[i] = __uint_as_float(v[i]);
                         }
-                    }
-                    refer(top);
-                    // ---- places whose values are not finite, for the rows that see them
-#pragma unroll 1
-                    for (int sw = 0; sw < S::kSlabs * 4; ++sw) {
-                        const int sl = sw >> 2, w = sw & 3;
-                        for (uint32_t left = odd[s_uses & 1][mine][sl][w]; left != 0; left &= left - 1) {
-                            const int key = w * 32 + __ffs(left) - 1, j = j0 + key;
-                            uint32_t raw_s;
-                            tmem_ld1(t_s + key, raw_s);
-                                                        const float p = (seen(w) >> (key & 31)) & 1u ? exp2_fast(fmaf(__uint_as_float(raw_s), scale2, -at_rest())) : 0.0f;
-                            const int64_t b = table[j / size];
-                            const T* v = static_cast<const T*>(a.vc) + b * g.vc_block_stride + (j % size) * g.vc_place_stride +
-                                         kvh * g.vc_head_stride + sl * 64;
-#pragma unroll 1
-                            for (int c = 0; c < 64; c += 16) {
-                                float o[16];
-                                tmem_ld16(t_o + sl * 64 + c, o);
+                        float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                                for (int i = 0; i < 16; ++i) {
-                                    const bool in = p > 0.0f && sl * 64 + c + i < g.head_dim;
-                                    o[i] += in ? p * to_f32(v[in ? c + i : 0]) : 0.0f;
-                                }
-                                tmem_st16(t_o + sl * 64 + c, o);
-                                tmem_wait_st();
+                        for (int i = 4; i < kHalf; ++i) {
+                            top[i & 3] = fmaxf(top[i & 3], x[i]);
+                        }
+                        refer(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+                        const float ref = at_rest();
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            weights(c, x + c * 32, ref);
+                        }
+                    } else {
+                        auto chunk = [&](int c, float (&x)[32]) {
+                            const uint32_t see = seen(2 * h + c);
+                            uint32_t v[32];
+                            tmem_ld32(t_h + c * 32, v);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                x[i] = (see >> i) & 1u ? __uint_as_float(v[i]) : -INFINITY;
+                            }
+                        };
+                        float top = -INFINITY;
+#pragma unroll 1
+                        for (int c = 0; c < 2; ++c) {
+                            float x[32];
+                            chunk(c, x);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                top = fmaxf(top, x[i]);
                             }
                         }
-                    }
-                    const float ref = at_rest();
-                    my_turn(t);
+                        refer(top);
+                        // ---- places whose values are not finite, for the rows that see them
 #pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        float x[32];
-                        chunk(c, x);
-                        weights(c, x, ref);
+                        for (int sw = 0; sw < S::kSlabs * 2; ++sw) {
+                            const int sl = sw >> 1, w = 2 * h + (sw & 1);
+                            for (uint32_t left = odd[s_uses & 1][mine][sl][w]; left != 0; left &= left - 1) {
+                                if (halves > 0) { // O is changed: after the last product
+                                    ok = mbar_wait(&o_done[s], (halves - 1) & 1, abort_flag, a.err, args.bound) && ok;
+                                    __syncwarp();
+                                    tc_fence_after();
+                                }
+                                const int key = w * 32 + __ffs(left) - 1, j = j0 + key;
+                                uint32_t raw_s;
+                                tmem_ld1(t_s + key, raw_s);
+                                const float p = (seen(w) >> (key & 31)) & 1u
+                                                    ? exp2_fast(fmaf(__uint_as_float(raw_s), scale2, -at_rest()))
+                                                    : 0.0f;
+                                const int64_t b = table[j / size];
+                                const T* v = static_cast<const T*>(a.vc) + b * g.vc_block_stride +
+                                             (j % size) * g.vc_place_stride + kvh * g.vc_head_stride + sl * 64;
+#pragma unroll 1
+                                for (int c = 0; c < 64; c += 16) {
+                                    float o[16];
+                                    tmem_ld16(t_o + sl * 64 + c, o);
+#pragma unroll
+                                    for (int i = 0; i < 16; ++i) {
+                                        const bool in = p > 0.0f && sl * 64 + c + i < g.head_dim;
+                                        o[i] += in ? p * to_f32(v[in ? c + i : 0]) : 0.0f;
+                                    }
+                                    tmem_st16(t_o + sl * 64 + c, o);
+                                    tmem_wait_st();
+                                }
+                            }
+                        }
+                        const float ref = at_rest();
+#pragma unroll 1
+                        for (int c = 0; c < 2; ++c) {
+                            float x[32];
+                            chunk(c, x);
+                            weights(c, x, ref);
+                        }
                     }
+                    z += (zz[0] + zz[1]) + (zz[2] + zz[3]);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(&p_full[s][h]);
                 }
-                pass_turn(t);
-                z += (zz[0] + zz[1]) + (zz[2] + zz[3]);
-                tmem_wait_st();
-                tc_fence_before();
-                mbar_arrive(&p_full[s]);
                 ++s_uses;
             }
             // ---- the item's end: O at rest, joined where the groups share rows, stored
             const int my_tiles = kTiles == 2 ? t1 - t0 : (t1 - t0 + 1 - s) / 2;
             if (my_tiles > 0) {
-                // s_uses counts this group's tiles, each with one product
-                ok = mbar_wait(&o_done[s], (s_uses - 1) & 1, abort_flag, a.err, args.bound) && ok;
+                // two products a tile: the last one completes phase 1
+                ok = mbar_wait(&o_done[s], 1, abort_flag, a.err, args.bound) && ok;
             }
             __syncwarp();
             tc_fence_after();
