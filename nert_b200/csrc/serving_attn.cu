@@ -20,7 +20,7 @@
 //
 // Within a CTA, WR x WK warps: row group x part of the tile's places. The warps of a row group run
 // the softmax on their own places and join at the end of the item. Tiles come by 16-byte cp.async
-// through a ring of NS stages, the addresses of a tile's rows looked up in the block table one tile
+// through a ring of NS stages, the addresses of a tile's rows looked up in the block table two tiles
 // ahead of its copies.
 
 #include "serving_attn.cuh"
@@ -95,21 +95,23 @@ struct Shape {
     static constexpr bool kF32Type = sizeof(T) == 4;
     static constexpr int kWarps = WR * WK, kThreads = 32 * kWarps;
     static constexpr int RT = 16 * WR;                    // rows of a block
-    static constexpr int KT = kF32Type ? 32 : 64;         // places of a tile
+    static constexpr int KT = kF32Type && DP > 64 ? 32 : 64; // places of a tile
     static constexpr int KW = KT / WK;                    // places of a warp
     static constexpr int kChunks = DP * sizeof(T) / 16;   // 16-byte chunks of a row
     static constexpr int kRow = DP * sizeof(T) + (kF32Type ? 16 : 0); // bytes of a row in shared memory
     static constexpr int kTile = KT * kRow;
     // stages of the ring: what fits beside Q
-    static constexpr int NS = DP == 64 ? 4 : DP == 128 || (WR == 1 && !kF32Type) ? 3 : 2;
+    static constexpr int NS = kF32Type && DP == 64 ? 3 : DP == 64 ? 4 : DP == 128 || (WR == 1 && !kF32Type) ? 3 : 2;
     static constexpr int kRing = NS * 2 * kTile;
     static constexpr int kQ = RT * kRow * (kF32Type ? 2 : 1);
     static constexpr int kJoin = WK * RT * DP * 4;        // the warps' sums, over the ring
     static constexpr int kSmem = (kRing > kJoin ? kRing : kJoin) + kQ + 1024;
+    // CTAs that shared memory lets an SM hold: registers are kept to what they leave
+    static constexpr int kPerSm = (kThreads == 128 || (WR == 2 && DP == 64)) && (kSmem + 8192) * 2 <= 227 * 1024 ? 2 : 1;
 };
 
 template <typename T, int DP, int WR, int WK>
-__global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(const __grid_constant__ TreeAttnArgs a, int group,
+__global__ void __launch_bounds__(32 * WR * WK, Shape<T, DP, WR, WK>::kPerSm) tree_attn_kernel(const __grid_constant__ TreeAttnArgs a, int group,
                                                                  int sms, float* part_o, float2* part_ml,
                                                                  uint32_t* tickets) {
     using S = Shape<T, DP, WR, WK>;
@@ -119,8 +121,9 @@ __global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(const __grid_co
     uint8_t* ring = attn_dyn;
     uint8_t* qs = attn_dyn + (S::kRing > S::kJoin ? S::kRing : S::kJoin);
     __shared__ int64_t red[NT / 32];
-    __shared__ int64_t k_at[NS][KT], v_at[NS][KT]; // element offsets of a tile's rows, -1: no such place
-    __shared__ int holes[NS][KT / 32];             // a place inside total has no block
+    // element offsets of the rows of the tiles in the ring and of the next, -1: no such place
+    __shared__ int64_t k_at[NS + 1][KT], v_at[NS + 1][KT];
+    __shared__ uint32_t valid_of[NS + 1][KT / 32]; // bits of the tiles' places that are there
     __shared__ unsigned long long odd_keys;        // places of the tile whose values are not finite
     __shared__ float2 warp_ml[WK][RT];
     __shared__ int64_t found[2];
@@ -166,7 +169,14 @@ __global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(const __grid_co
         const int32_t* table = a.table + r * g.table_stride;
 
         __syncthreads(); // the last item's use of shared memory is over
+        // block of place j of this request, for the row addresses of a tile; -1: none there
+        auto look_up = [&](int tile) -> int {
+            const int j = tile * KT + tid;
+            return tid < KT && tile < t_end && j < rq.total ? table[j / static_cast<int>(g.block_size)] : -1;
+        };
+        int next = look_up(t_begin);
         // ---- Q rows into shared memory, zero past the block's rows and head_dim
+#pragma unroll 1
         for (int i = tid; i < RT * S::kChunks; i += NT) {
             const int row = i / S::kChunks, ch = i - row * S::kChunks;
             constexpr int E = 16 / sizeof(T);
@@ -204,36 +214,28 @@ __global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(const __grid_co
             }
         }
 
-        // block of place j of this request, for the row addresses of a tile; -1: none
-        auto look_up = [&](int tile) -> int {
-            const int j = tile * KT + tid;
-            if (tid >= KT || tile >= t_end || j >= rq.total) {
-                return -2;
-            }
-            return table[j / static_cast<int>(g.block_size)];
-        };
         auto place_rows = [&](int tile, int block) {
-            if (tid < KT) {
-                const int st = (tile - t_begin) % NS;
+            if (tid < KT && tile < t_end) {
+                const int at = tile % (NS + 1), j = tile * KT + tid;
                 int64_t ka = -1, va = -1;
-                const bool hole = block != -2 && (block < 0 || block >= g.num_blocks);
-                const uint32_t any = __ballot_sync(0xffffffffu, hole);
+                const bool there = block >= 0 && block < g.num_blocks;
+                const uint32_t valid = __ballot_sync(0xffffffffu, there);
                 if (lane == 0) {
-                    holes[st][warp] = any != 0;
+                    valid_of[at][warp] = valid;
                 }
-                bad |= hole;
-                if (block >= 0 && block < g.num_blocks) {
-                    const int64_t p = (tile * KT + tid) % static_cast<int>(g.block_size);
+                bad |= !there && j < rq.total;
+                if (there) {
+                    const int p = j % static_cast<int>(g.block_size);
                     ka = block * g.kc_block_stride + p * g.kc_place_stride + kvh * g.kc_head_stride;
                     va = block * g.vc_block_stride + p * g.vc_place_stride + kvh * g.vc_head_stride;
                 }
-                k_at[st][tid] = ka;
-                v_at[st][tid] = va;
+                k_at[at][tid] = ka;
+                v_at[at][tid] = va;
             }
         };
         auto copy_tile = [&](int tile) {
             if (tile < t_end) {
-                const int st = (tile - t_begin) % NS;
+                const int st = tile % NS, at = tile % (NS + 1);
                 const uint32_t dst = smem_u32(ring + st * 2 * S::kTile);
                 constexpr int kPer = NT / S::kChunks > 0 ? NT / S::kChunks : 1; // rows of one pass
                 static_assert(NT % S::kChunks == 0 && KT % kPer == 0, "the threads cover whole rows");
@@ -241,10 +243,10 @@ __global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(const __grid_co
                 const bool in = ch * static_cast<int>(16 / sizeof(T)) < D;
                 const T* kc = static_cast<const T*>(a.kc) + ch * (16 / sizeof(T));
                 const T* vc = static_cast<const T*>(a.vc) + ch * (16 / sizeof(T));
-#pragma unroll
+#pragma unroll 4
                 for (int i = 0; i < KT / kPer; ++i) {
                     const int row = row0 + i * kPer;
-                    const int64_t ka = k_at[st][row], va = v_at[st][row];
+                    const int64_t ka = k_at[at][row], va = v_at[at][row];
                     const uint32_t off = row * S::kRow + (S::kF32Type ? ch * 16 : ((ch ^ (row & 7)) << 4));
                     const bool live = in && ka >= 0;
                     cp_async16(dst + off, kc + (live ? ka : 0), live);
@@ -254,15 +256,9 @@ __global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(const __grid_co
             cp_commit();
         };
 
-#pragma unroll
-        for (int i = 0; i < NS - 1; ++i) {
-            place_rows(t_begin + i, look_up(t_begin + i));
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < NS - 1; ++i) {
-            copy_tile(t_begin + i);
-        }
+        place_rows(t_begin, next);
+        next = look_up(t_begin + 1);
+        __syncthreads(); // Q is there
 
         uint32_t qf[S::kF32Type ? 1 : DP / 16][4];
         if constexpr (!S::kF32Type) {
@@ -279,43 +275,58 @@ __global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(const __grid_co
         }
         float m0 = -INFINITY, m1 = -INFINITY, z0 = 0.0f, z1 = 0.0f; // of rows gq and gq + 8, this thread's columns
 
-        for (int tile = t_begin; tile < t_end; ++tile) {
-            const int st = (tile - t_begin) % NS;
-            const int next = look_up(tile + NS - 1);
-            cp_wait<NS - 2>();
-            __syncthreads(); // the tile has landed; the stage before it is free
-            if (tid == 0) {
-                odd_keys = 0;
+        // The first NS - 1 rounds only fill the ring. A CTA may meet few tiles, so what runs once is
+        // kept small: its instructions come from L2.
+#pragma unroll 1
+        for (int tile = t_begin - (NS - 1); tile < t_end; ++tile) {
+            if (tile >= t_begin) {
+                cp_wait<NS - 2>();
             }
+            __syncthreads(); // the tile has landed, the stage of the one before is free, the next addresses are there
+            copy_tile(tile + NS - 1);
+            place_rows(tile + NS, next);
+            next = look_up(tile + NS + 1);
+            if (tile < t_begin) {
+                continue;
+            }
+            const int st = tile % NS, at = tile % (NS + 1);
             const int j0 = tile * KT;
-            const bool plain = j0 + KT <= old && holes[st][0] == 0 && holes[st][KT / 32 - 1] == 0;
+            bool plain = j0 + KT <= old;
+#pragma unroll
+            for (int i = 0; i < KT / 32; ++i) {
+                plain = plain && valid_of[at][i] == 0xffffffffu;
+            }
             uint8_t* kt = ring + st * 2 * S::kTile;
             uint8_t* vt = kt + S::kTile;
+            uint64_t odd = 0; // places whose values are not finite
             if (!plain) {
                 // Values that are not finite would reach the rows that do not
                 // see them as 0 * inf: taken out of the tile here, added for the rows that do below.
+                if (tid == 0) {
+                    odd_keys = 0;
+                }
                 __syncthreads();
-                for (int i = tid; i < KT * (S::kRow / 16); i += NT) {
-                    const int row = i / (S::kRow / 16);
-                    const T* e = reinterpret_cast<const T*>(vt + row * S::kRow + (i - row * (S::kRow / 16)) * 16);
-                    if (S::kF32Type && (i - row * (S::kRow / 16)) >= S::kChunks) {
-                        continue; // the padding of a row
-                    }
-                    bool odd = false;
+#pragma unroll 1
+                for (int i = tid; i < KT * S::kChunks; i += NT) {
+                    const int row = i / S::kChunks, ch = i - row * S::kChunks;
+                    const T* e = reinterpret_cast<const T*>(vt + row * S::kRow + ch * 16);
+                    bool found_odd = false;
 #pragma unroll
                     for (int x = 0; x < static_cast<int>(16 / sizeof(T)); ++x) {
-                        odd |= !isfinite(to_f32(e[x]));
+                        found_odd |= !isfinite(to_f32(e[x]));
                     }
-                    if (odd) {
+                    if (found_odd) {
                         atomicOr(&odd_keys, 1ull << row);
                     }
                 }
                 __syncthreads();
-                if (odd_keys != 0) {
-                    for (int i = tid; i < KT * (S::kRow / 16); i += NT) {
-                        const int row = i / (S::kRow / 16);
-                        if ((odd_keys >> row) & 1) {
-                            *reinterpret_cast<uint4*>(vt + i * 16) = make_uint4(0, 0, 0, 0);
+                odd = odd_keys;
+                if (odd != 0) {
+#pragma unroll 1
+                    for (int i = tid; i < KT * S::kChunks; i += NT) {
+                        const int row = i / S::kChunks, ch = i - row * S::kChunks;
+                        if ((odd >> row) & 1) {
+                            *reinterpret_cast<uint4*>(vt + row * S::kRow + ch * 16) = make_uint4(0, 0, 0, 0);
                         }
                     }
                     __syncthreads();
@@ -383,19 +394,17 @@ __global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(const __grid_co
                     }
                 }
             } else {
+                // the warp's places (at most 32) that the rows' tokens see
+                const int first_col = wk * KW;
+                const uint32_t there = valid_of[at][first_col / 32] >> (first_col % 32);
+                const uint32_t see0 = tok0 >= 0 ? there & see_bits(mask0, g.mask_words, tok0, j0 + first_col - old) : 0u;
+                const uint32_t see1 = tok1 >= 0 ? there & see_bits(mask1, g.mask_words, tok1, j0 + first_col - old) : 0u;
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int col = wk * KW + nb * 8 + 2 * cq + (e & 1);
-                        const int j = j0 + col, k = j - old;
-                        const int tok = e < 2 ? tok0 : tok1;
-                        bool see = tok >= 0 && j < rq.total && k_at[st][col] >= 0;
-                        if (see && k >= 0) {
-                            const uint32_t* mk = e < 2 ? mask0 : mask1;
-                            see = mk == nullptr ? k <= tok : (k >> 5) < g.mask_words && ((mk[k >> 5] >> (k & 31)) & 1u);
-                        }
-                        s[nb][e] = see ? s[nb][e] * scale2 : -INFINITY;
+                        const uint32_t see = e < 2 ? see0 : see1;
+                        s[nb][e] = (see >> (nb * 8 + 2 * cq + (e & 1))) & 1u ? s[nb][e] * scale2 : -INFINITY;
                     }
                 }
             }
@@ -482,37 +491,33 @@ __global__ void __launch_bounds__(32 * WR * WK) tree_attn_kernel(const __grid_co
                     }
                 }
             }
-            if (!plain && odd_keys != 0) {
-                // values that are not finite, for the rows that see them
+            // values that are not finite, for the rows that see them
+            uint64_t mine = (odd >> (wk * KW)) & ((uint64_t{1} << KW) - 1);
+#pragma unroll 1
+            for (; mine != 0; mine &= mine - 1) { // the same for the whole warp
+                const int col = __ffsll(static_cast<long long>(mine)) - 1, holder = (lane & 28) | ((col & 7) >> 1);
+                float p0 = 0.0f, p1 = 0.0f;
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
+                    if (nb == col >> 3) {
+                        p0 = (col & 1) != 0 ? s[nb][1] : s[nb][0];
+                        p1 = (col & 1) != 0 ? s[nb][3] : s[nb][2];
+                    }
+                }
+                p0 = __shfl_sync(0xffffffffu, p0, holder);
+                p1 = __shfl_sync(0xffffffffu, p1, holder);
+                const T* v = static_cast<const T*>(a.vc) + v_at[at][wk * KW + col] + 2 * cq;
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        const int col = wk * KW + nb * 8 + c;
-                        if (((odd_keys >> col) & 1) == 0) {
-                            continue; // the same for the whole warp
-                        }
-                        const float p0 = __shfl_sync(0xffffffffu, s[nb][c & 1], (lane & 28) | (c >> 1));
-                        const float p1 = __shfl_sync(0xffffffffu, s[nb][2 + (c & 1)], (lane & 28) | (c >> 1));
-                        const T* v = static_cast<const T*>(a.vc) + v_at[st][col];
-#pragma unroll
-                        for (int i = 0; i < DP / 8; ++i) {
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const int d = i * 8 + 2 * cq + e;
-                                if (d < D) {
-                                    const float x = to_f32(v[d]);
-                                    o[i][e] += p0 > 0.0f ? p0 * x : 0.0f;
-                                    o[i][2 + e] += p1 > 0.0f ? p1 * x : 0.0f;
-                                }
-                            }
-                        }
+                for (int i = 0; i < DP / 8; ++i) {
+                    if (i * 8 < D) {
+                        const float x0 = to_f32(v[i * 8]), x1 = to_f32(v[i * 8 + 1]);
+                        o[i][0] += p0 > 0.0f ? p0 * x0 : 0.0f;
+                        o[i][1] += p0 > 0.0f ? p0 * x1 : 0.0f;
+                        o[i][2] += p1 > 0.0f ? p1 * x0 : 0.0f;
+                        o[i][3] += p1 > 0.0f ? p1 * x1 : 0.0f;
                     }
                 }
             }
-            place_rows(tile + NS - 1, next);
-            __syncthreads(); // every warp is done with the stage; the next tile's addresses are there
-            copy_tile(tile + NS - 1);
         }
         cp_wait<0>();
         __syncthreads();
@@ -646,7 +651,7 @@ void tree_attention(nb2_device* dev, TreeAttnArgs a) {
         return;
     }
     a.err = dev->err_word;
-    if (tree_attention_tc_takes(a)) {
+    if (tree_attention_tc_takes(a, dev->num_sms)) {
         tree_attention_tc(dev, a);
     } else if (a.g.dtype == kF32) {
         pick_dim<float>(dev, a);

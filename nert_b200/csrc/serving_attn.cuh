@@ -76,6 +76,23 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+// Bits of places k0 .. k0 + 31, counted from the first new token, that a row's token sees.
+__device__ __forceinline__ uint32_t see_bits(const uint32_t* mask, int64_t words, int tok, int k0) {
+    if (k0 <= -32) {
+        return 0xffffffffu;
+    }
+    if (mask == nullptr) { // a chain: up to the token itself
+        const int n = tok - k0 + 1;
+        return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+    }
+    if (k0 < 0) {
+        return (mask[0] << -k0) | ((1u << -k0) - 1u);
+    }
+    const int w = k0 >> 5, s = k0 & 31;
+    const uint32_t lo = w < words ? mask[w] : 0u, hi = w + 1 < words ? mask[w + 1] : 0u;
+    return __funnelshift_r(lo, hi, s);
+}
+
 // ---- the join ------------------------------------------------------------------
 
 // Elements d .. d + 3 of a finished row (unnormalised sums x, maximum m in base 2, sum of weights z).
@@ -193,8 +210,8 @@ struct Span {
     int64_t request_unit; // first unit of that request
 };
 
-// Spans shorter than kMinSpan units are not made while `least` CTAs have one: more CTAs an SM would then read no
-// faster, and each adds a piece to the join.
+// Spans shorter than kMinSpan units are not made once `least` CTAs have one: each adds a piece to a join, whose pieces
+// take about a third of a tile each.
 constexpr int kMinSpan = 4;
 
 template <int RT, int KT, int NT>
@@ -255,7 +272,7 @@ __device__ __forceinline__ Span find_span(const TreeAttnArgs& a, int group, int 
 }
 
 // The tensor-core kernel for many rows (serving_attn_tc.cu): whether it takes the call, and the call.
-bool tree_attention_tc_takes(const TreeAttnArgs& a);
+bool tree_attention_tc_takes(const TreeAttnArgs& a, int sms);
 void tree_attention_tc(nb2_device* dev, const TreeAttnArgs& a);
 
 } // namespace nb2

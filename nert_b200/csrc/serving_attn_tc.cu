@@ -162,23 +162,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     }
 }
 
-// Bits of places k0 .. k0 + 31, counted from the first new token, that a row's token sees.
-__device__ __forceinline__ uint32_t see_bits(const uint32_t* mask, int64_t words, int tok, int k0) {
-    if (k0 <= -32) {
-        return 0xffffffffu;
-    }
-    if (mask == nullptr) { // a chain: up to the token itself
-        const int n = tok - k0 + 1;
-        return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
-    }
-    if (k0 < 0) {
-        return (mask[0] << -k0) | ((1u << -k0) - 1u);
-    }
-    const int w = k0 >> 5, s = k0 & 31;
-    const uint32_t lo = w < words ? mask[w] : 0u, hi = w + 1 < words ? mask[w + 1] : 0u;
-    return __funnelshift_r(lo, hi, s);
-}
-
 struct TcArgs {
     TreeAttnArgs a;
     int group;
@@ -213,7 +196,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tc_dyn) + 1023) & ~uintptr_t(1023));
     uint8_t* ks = qs + S::kQ;
     uint8_t* vs = ks + NS * S::kKV;
-    __shared__ uint64_t k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], s_full[2][2], p_full[2][2], o_done[2], q_full,
+    __shared__ uint64_t k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], s_full[2][2], p_full[2][2], o_done[2][2], q_full,
         drain;
     __shared__ int64_t red[kTcThreads / 32], found[2];
     __shared__ uint32_t tmem_slot;
@@ -238,8 +221,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             for (int h = 0; h < 2; ++h) {
                 mbar_init(&s_full[i][h], 1);
                 mbar_init(&p_full[i][h], kTile);
+                mbar_init(&o_done[i][h], 1);
             }
-            mbar_init(&o_done[i], 1);
         }
         mbar_init(&q_full, kSoftmax);
         mbar_init(&drain, 2);
@@ -255,7 +238,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         prefetch_tmap(&k_map);
         prefetch_tmap(&v_map);
     }
-    const Span span = find_span<RT, kTile, kTcThreads>(a, group, gridDim.x, red, found, bad);
+    const Span span = find_span<RT, kTile, kTcThreads>(a, group, 1, red, found, bad);
     spare_tokens<T>(a, tid, kTcThreads);
     tc_fence_before();
     __syncthreads();
@@ -398,13 +381,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             for (int c = 0; c < kHalf / 16; ++c) {
                                 mma_f16_ta(t_o, t_s + h * kHalf + c * 8, sdesc_128(v + c * 2048, S::kSlab), idesc_o);
                             }
-                            mma_commit(&o_done[s]);
+                            mma_commit(&o_done[s][h]);
                             if (h == 1) {
                                 mma_commit(&v_empty[st]);
                             }
                         }
                         if (i + kStep < nt) {
-                            ok = ok && wait(&o_done[s], h); // two products a tile: the first completes phase 0, the second 1
+                            ok = ok && wait(&o_done[s][h], uses & 1);
                             scores(i + kStep, h);
                         }
                     }
@@ -505,6 +488,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             float m = -INFINITY, z = 0.0f; // reference and sum of this row
             bool ok = !*abort_flag;
             uint32_t halves = 0; // of this item, whose weights this thread has given
+            // After the product of the last weights that this thread has given. (A barrier for each half: the phase before the one
+            // awaited is then always over, its half's next scores having been made after it.)
+            auto rest = [&] {
+                if (halves > 0) {
+                    const uint32_t h = (halves - 1) & 1;
+                    ok = mbar_wait(&o_done[s][h], (s_uses - (h == 1 ? 1 : 0)) & 1, abort_flag, a.err, args.bound) && ok;
+                    __syncwarp();
+                    tc_fence_after();
+                }
+            };
             // The reference for scores whose largest is `raw`: O and the sum move to a new one where it is too far below,
             // after the last product.
             auto refer = [&](float raw) {
@@ -512,11 +505,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (!__any_sync(0xffffffffu, now > m + 8.0f)) {
                     return;
                 }
-                if (halves > 0) {
-                    ok = mbar_wait(&o_done[s], (halves - 1) & 1, abort_flag, a.err, args.bound) && ok;
-                    __syncwarp();
-                    tc_fence_after();
-                }
+                rest();
                 const float to = fmaxf(m, now), keep = to == -INFINITY ? 1.0f : exp2_fast(m - to);
                 if (__any_sync(0xffffffffu, m > -INFINITY)) {
 #pragma unroll 1
@@ -665,11 +654,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         for (int sw = 0; sw < S::kSlabs * 2; ++sw) {
                             const int sl = sw >> 1, w = 2 * h + (sw & 1);
                             for (uint32_t left = odd[s_uses & 1][mine][sl][w]; left != 0; left &= left - 1) {
-                                if (halves > 0) { // O is changed: after the last product
-                                    ok = mbar_wait(&o_done[s], (halves - 1) & 1, abort_flag, a.err, args.bound) && ok;
-                                    __syncwarp();
-                                    tc_fence_after();
-                                }
+                                rest(); // O is changed
                                 const int key = w * 32 + __ffs(left) - 1, j = j0 + key;
                                 uint32_t raw_s;
                                 tmem_ld1(t_s + key, raw_s);
@@ -711,8 +696,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // ---- the item's end: O at rest, joined where the groups share rows, stored
             const int my_tiles = kTiles == 2 ? t1 - t0 : (t1 - t0 + 1 - s) / 2;
             if (my_tiles > 0) {
-                // two products a tile: the last one completes phase 1
-                ok = mbar_wait(&o_done[s], 1, abort_flag, a.err, args.bound) && ok;
+                for (int h = 0; h < 2; ++h) {
+                    ok = mbar_wait(&o_done[s][h], (s_uses - 1) & 1, abort_flag, a.err, args.bound) && ok;
+                }
             }
             __syncwarp();
             tc_fence_after();
@@ -938,7 +924,7 @@ void pick_tiles(nb2_device* dev, const TreeAttnArgs& a) {
 
 } // namespace
 
-bool tree_attention_tc_takes(const TreeAttnArgs& a) {
+bool tree_attention_tc_takes(const TreeAttnArgs& a, int sms) {
     const nb2_tree_attn_geom& g = a.g;
     const int64_t rows = std::min(g.max_new, g.tokens) * (g.q_heads / g.kv_heads);
     const bool page = g.block_size >= 8 && (g.block_size & (g.block_size - 1)) == 0;
@@ -948,7 +934,11 @@ bool tree_attention_tc_takes(const TreeAttnArgs& a) {
                       g.vc_head_stride}) {
         strides = strides && s > 0 && s < most;
     }
-    return g.dtype != kF32 && rows > kTcRows && g.head_dim >= 64 && g.head_dim <= 128 && page && strides && g.num_blocks > 0;
+    // Up to 64 rows with less than a tile a CTA: an item's beginning and end cost more than its products (2 requests of
+    // 48 rows over 3,400 places 40 us here, 22 us there; 7 of them over 3,000 places 31 and 51 us).
+    const int64_t tiles = g.batch * g.kv_heads * ((g.table_blocks * g.block_size + kTile - 1) / kTile);
+    const bool enough = rows > 64 || (rows > kTcRows && tiles > sms);
+    return g.dtype != kF32 && enough && g.head_dim >= 64 && g.head_dim <= 128 && page && strides && g.num_blocks > 0;
 }
 
 void tree_attention_tc(nb2_device* dev, const TreeAttnArgs& a) {
