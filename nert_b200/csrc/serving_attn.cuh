@@ -203,16 +203,21 @@ __device__ __forceinline__ void spare_tokens(const TreeAttnArgs& a, int tid, int
     }
 }
 
+// Spans shorter than kMinSpan units are not made once `least` CTAs have one: each adds a piece to a join, whose pieces
+// take about a third of a tile each.
+constexpr int kMinSpan = 4;
+
 // This CTA's span of the W units, and the request that its first unit is in. All NT threads.
 struct Span {
     int64_t W, grid, w0, w1;
     int request;          // holds unit w0
     int64_t request_unit; // first unit of that request
+    __device__ __forceinline__ void set(int64_t cta, int least) {
+        grid = min(static_cast<int64_t>(gridDim.x), max(W / kMinSpan, min(W, static_cast<int64_t>(least)))); // none is empty
+        w0 = cta < grid ? cta * W / grid : 0;
+        w1 = cta < grid ? (cta + 1) * W / grid : 0;
+    }
 };
-
-// Spans shorter than kMinSpan units are not made once `least` CTAs have one: each adds a piece to a join, whose pieces
-// take about a third of a tile each.
-constexpr int kMinSpan = 4;
 
 template <int RT, int KT, int NT>
 __device__ __forceinline__ Span find_span(const TreeAttnArgs& a, int group, int least, int64_t* red, int64_t* found,
@@ -221,6 +226,23 @@ __device__ __forceinline__ Span find_span(const TreeAttnArgs& a, int group, int 
     const int B = static_cast<int>(a.g.batch);
     const int64_t cta = blockIdx.x;
     Span s{};
+    if (B <= 32) { // every warp for itself: no barrier
+        const Request q = lane < B ? request_at<RT, KT>(a, lane, group) : Request{};
+        bad |= q.bad;
+        const int64_t u = q.units(a.g.kv_heads);
+        int64_t inc = u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t up = __shfl_up_sync(0xffffffffu, inc, o);
+            inc += lane >= o ? up : 0;
+        }
+        s.W = __shfl_sync(0xffffffffu, inc, 31);
+        s.set(cta, least);
+        const uint32_t hit = __ballot_sync(0xffffffffu, s.w0 < s.w1 && inc - u <= s.w0 && s.w0 < inc);
+        s.request = hit != 0 ? __ffs(hit) - 1 : 0;
+        s.request_unit = __shfl_sync(0xffffffffu, inc - u, s.request);
+        return s;
+    }
     int64_t mine = 0; // units of request tid
     for (int r = tid; r < B; r += NT) {
         const Request q = request_at<RT, KT>(a, r, group);
@@ -229,12 +251,10 @@ __device__ __forceinline__ Span find_span(const TreeAttnArgs& a, int group, int 
         mine = r == tid ? s.W : mine;
     }
     s.W = block_sum<NT>(s.W, red);
-    s.grid = min(static_cast<int64_t>(gridDim.x), max(s.W / kMinSpan, min(s.W, static_cast<int64_t>(least)))); // no span is empty
-    if (cta >= s.grid) {
+    s.set(cta, least);
+    if (s.w0 == s.w1) {
         return s;
     }
-    s.w0 = cta * s.W / s.grid;
-    s.w1 = (cta + 1) * s.W / s.grid;
     int64_t base = 0;
     for (int c = 0; c < B; c += NT) {
         const int64_t u = c == 0 ? mine : c + tid < B ? request_at<RT, KT>(a, c + tid, group).units(a.g.kv_heads) : 0;

@@ -306,8 +306,13 @@ void launch_logits(nb2_device* dev, const LogitsArgs& a) {
     if (chunks > 65535) {
         fail(kStatusUnsupported, "LogitsProcess: too many tokens");
     }
-    // rows of a CTA: as many as leave each SM four CTAs to run one after another or at once
-    const int64_t rows = std::min<int64_t>(kMaxRows, std::max<int64_t>(1, a.g.rows * chunks / (4 * dev->num_sms)));
+    // rows of a CTA: as many as leave each SM four CTAs to run one after another or at once, and whole requests where
+    // those have so few rows (a CTA that meets a second request walks lists twice)
+    int64_t rows = std::min<int64_t>(kMaxRows, std::max<int64_t>(1, a.g.rows * chunks / (4 * dev->num_sms)));
+    const int64_t each = a.g.requests > 0 ? a.g.rows / a.g.requests : 1;
+    if (each > 1 && rows > each) {
+        rows = rows / each * each;
+    }
     const dim3 grid(static_cast<unsigned>((a.g.rows + rows - 1) / rows), static_cast<unsigned>(chunks));
     kernel<<<grid, kLogitThreads, smem, dev->stream>>>(a, static_cast<int>(rows));
     check_cuda(cudaGetLastError(), "logits launch");
