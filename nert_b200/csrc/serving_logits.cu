@@ -15,7 +15,7 @@
 // every row of the request is streamed, the next row's loads in flight, every element through the same
 // few instructions: x * (x > 0 ? 1/rep : rep or 1) + word.
 // Measured (408 rows of 128,000 tokens in bfloat16 to float32, 313 MB, 24 requests of up to 8,000
-// tokens): 91 us, 3.5 TB/s; 67 us with the output lists alone. Rules only where a bitmap has a bit, inside the stream (some lane of nearly every warp
+// tokens): 82 us, 3.9 TB/s. Rules only where a bitmap has a bit, inside the stream (some lane of nearly every warp
 // has one; 37 instructions an element): 115 us. Plain stream, then single stores at the touched
 // tokens (each a read and a partial write of a sector in L2): 150 us.
 
@@ -66,7 +66,7 @@ __device__ __forceinline__ void walk_list(const int32_t* ids, int lo, int hi, in
 
 // kLevel: every row starts on a whole pack, in the logits and in the results.
 template <typename TI, typename TO, bool kBias, bool kLevel>
-__global__ void __launch_bounds__(kLogitThreads) logits_kernel(const __grid_constant__ LogitsArgs a, int rows_per_cta) {
+__global__ void __launch_bounds__(kLogitThreads, kLevel ? 5 : 1) logits_kernel(const __grid_constant__ LogitsArgs a, int rows_per_cta) {
     extern __shared__ uint32_t logit_smem[];
     // logits of a thread and step: the wider side is 16 bytes, so that a warp's loads and stores have no gaps
     constexpr int V = 16 / (sizeof(TI) > sizeof(TO) ? sizeof(TI) : sizeof(TO));

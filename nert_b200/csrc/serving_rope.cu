@@ -6,14 +6,13 @@
 // once in and once out. The angles come as a table of cosines and sines in 32
 // bits (the caller's: any base, scaling or length rule), gathered by position.
 //
-// A thread owns V consecutive frequencies of one token and walks over some of
-// its heads, so cos and sin are loaded once for all of them; the next head's two
-// V-element packs are loaded before the present one is turned and stored. Both halves
-// of every pair are read before either is written, which is what makes the
-// in-place form safe. The walk is a rolled loop: what bounds the kernel is how many loads an
-// SM holds in flight, and 64 registers a thread (1,024 threads of 64 bytes each) took 76 us
-// for 297 MB (16,001 tokens, 28 + 4 + 4 heads of 128 in bfloat16; 3.9 TB/s), four heads unrolled in
-// 122 registers 117 us, 48 registers with spills 125 us.
+// A CTA takes heads of q, of k or of v. A thread owns V consecutive frequencies of one token and walks over some of
+// the token's heads, so cos and sin are loaded once for all of them; the next head's two V-element packs are loaded
+// before the present one is turned and stored. Both halves of every pair are read before either is written, which
+// is what makes the in-place form safe. What bounds the kernel is how many loads an SM holds in flight, that is,
+// registers: a rolled walk over one tensor needs at most 64 (1,024 threads of 64 bytes each, nothing spilled).
+// Measured at 16,001 tokens, 28 + 4 + 4 heads of 128 in bfloat16 (297 MB): 56 us, 5.3 TB/s. Walking over all three
+// tensors in the same registers took 72 us, four heads unrolled in 122 registers 117 us, 48 registers with spills 94 us.
 
 #include "serving.cuh"
 
@@ -22,57 +21,72 @@ namespace nb2 {
 namespace {
 
 constexpr int kRopeThreads = 256;
-constexpr int kWalk = 4;
+// Heads of a thread where there are tokens enough: the table's rows are read that much less often. 16-bit types: 8 heads
+// 56 us, 4 heads 60, 2 heads 69; float32 (6,304 tokens, 12 + 12 heads of 64): 2 heads 16 us, 4 heads 18, 8 heads 20.
+constexpr int walk_of(size_t bytes) { return bytes == 2 ? 8 : 2; }
+
+// How the heads of one tensor are spread over CTAs.
+struct Spread {
+    int heads;
+    int groups; // threads that share a token's heads at one lane
+    int tokens; // of a CTA
+    int64_t ctas;
+};
 
 template <typename T, int V, bool kPairs, bool kOneAxis>
 __global__ void __launch_bounds__(kRopeThreads, 4)
-    rope_kernel(const __grid_constant__ RopeArgs a, int lanes, int groups, int tokens_per_cta) {
+    rope_kernel(const __grid_constant__ RopeArgs a, int lanes, const __grid_constant__ Spread sq,
+                const __grid_constant__ Spread sk) {
     using P = Pack<T, V>;
     const nb2_rope_geom& g = a.g;
-    const int work = lanes * groups;
+    const int64_t cta = blockIdx.x;
+    const int role = cta < sq.ctas ? 0 : cta < sq.ctas + sk.ctas ? 1 : 2; // q, k, v
+    const int heads = role == 0 ? sq.heads : sk.heads, groups = role == 0 ? sq.groups : sk.groups;
+    const int tokens = role == 0 ? sq.tokens : sk.tokens, work = lanes * groups;
     const int local = static_cast<int>(threadIdx.x) / work;
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * tokens_per_cta + local;
-    if (local >= tokens_per_cta || t >= g.tokens) {
+    const int64_t t = (role == 0 ? cta : role == 1 ? cta - sq.ctas : cta - sq.ctas - sk.ctas) * tokens + local;
+    if (local >= tokens || t >= g.tokens) {
         return;
     }
     const int half = static_cast<int>(g.rot_dim / 2);
     const int turn = half / V; // lanes that turn pairs; the rest copy what is past rot_dim
-    const int q_heads = static_cast<int>(g.q_heads), kv_heads = static_cast<int>(g.kv_heads);
-    const int heads = q_heads + kv_heads + (a.v != nullptr ? kv_heads : 0);
     const int w = static_cast<int>(threadIdx.x) - local * work;
     const int group = w / lanes, lane = w - group * lanes;
-    const bool turns = lane < turn;
+    const bool turns = role < 2 && lane < turn;
     // element offsets of the two packs in a head
-    const int e0 = !turns ? static_cast<int>(g.rot_dim) + (lane - turn) * 2 * V : kPairs ? lane * 2 * V : lane * V;
-    const int e1 = turns && !kPairs ? half + e0 : e0 + V;
+    const int e0 = lane >= turn ? static_cast<int>(g.rot_dim) + (lane - turn) * 2 * V : kPairs ? lane * 2 * V : lane * V;
+    const int e1 = lane < turn && !kPairs ? half + e0 : e0 + V;
 
-    auto source = [&](int h) -> const T* { // a row: one head of the token, over q's, k's and v's heads
-        if (h < q_heads) {
-            return static_cast<const T*>(a.q) + t * g.q_stride + h * g.q_head_stride;
+    const int64_t src_head = role == 0 ? g.q_head_stride : role == 1 ? g.k_head_stride : g.v_head_stride;
+    const T* src = (role == 0   ? static_cast<const T*>(a.q) + t * g.q_stride
+                    : role == 1 ? static_cast<const T*>(a.k) + t * g.k_stride
+                                : static_cast<const T*>(a.v) + t * g.v_stride) +
+                   group * src_head;
+    P x0 = *reinterpret_cast<const P*>(src + e0), x1 = *reinterpret_cast<const P*>(src + e1);
+
+    // where the heads go: out, and the token's place in a cache (null: nowhere)
+    T *out = nullptr, *cache = nullptr;
+    int64_t out_head = 0, cache_head = 0;
+    if (role == 0) {
+        out_head = g.qo_head_stride;
+        out = static_cast<T*>(a.q_out) + t * g.qo_stride;
+    } else {
+        if (role == 1 && a.k_out != nullptr) {
+            out_head = g.ko_head_stride;
+            out = static_cast<T*>(a.k_out) + t * g.ko_stride;
         }
-        h -= q_heads;
-        if (h < kv_heads) {
-            return static_cast<const T*>(a.k) + t * g.k_stride + h * g.k_head_stride;
-        }
-        return static_cast<const T*>(a.v) + t * g.v_stride + (h - kv_heads) * g.v_head_stride;
-    };
-    P x0, x1;
-    {
-        const T* row = source(group);
-        x0 = *reinterpret_cast<const P*>(row + e0);
-        x1 = *reinterpret_cast<const P*>(row + e1);
-    }
-    int64_t k_at = -1, v_at = -1; // the token's place in the caches
-    if (a.slots != nullptr) {
-        const int slot = a.slots[t];
+        const int slot = a.slots != nullptr ? a.slots[t] : -1;
         if (slot >= 0) {
             const int size = static_cast<int>(g.block_size);
             const int block = slot / size, place = slot - block * size;
-            if (block < g.num_blocks) {
-                k_at = block * g.kc_block_stride + place * g.kc_place_stride;
-                v_at = block * g.vc_block_stride + place * g.vc_place_stride;
-            } else {
+            if (block >= g.num_blocks) {
                 record_error(a.err, kDevIndexOutOfRange);
+            } else if (role == 1) {
+                cache_head = g.kc_head_stride;
+                cache = static_cast<T*>(a.k_cache) + block * g.kc_block_stride + place * g.kc_place_stride;
+            } else {
+                cache_head = g.vc_head_stride;
+                cache = static_cast<T*>(a.v_cache) + block * g.vc_block_stride + place * g.vc_place_stride;
             }
         }
     }
@@ -106,12 +120,12 @@ __global__ void __launch_bounds__(kRopeThreads, 4)
 #pragma unroll 1
     for (int h = group; h < heads; h += groups) {
         P n0, n1;
+        src += groups * src_head;
         if (h + groups < heads) {
-            const T* row = source(h + groups);
-            n0 = *reinterpret_cast<const P*>(row + e0);
-            n1 = *reinterpret_cast<const P*>(row + e1);
+            n0 = *reinterpret_cast<const P*>(src + e0);
+            n1 = *reinterpret_cast<const P*>(src + e1);
         }
-        if (turns && h < q_heads + kv_heads) {
+        if (turns) {
             if constexpr (kPairs) { // pair j: elements 2j, 2j + 1 of the two packs together
                 T x[2 * V];
 #pragma unroll
@@ -139,22 +153,15 @@ __global__ void __launch_bounds__(kRopeThreads, 4)
                 }
             }
         }
-        auto store = [&](T* row) {
+        if (out != nullptr) {
+            T* row = out + h * out_head;
             *reinterpret_cast<P*>(row + e0) = x0;
             *reinterpret_cast<P*>(row + e1) = x1;
-        };
-        const int hk = h - q_heads;
-        if (hk < 0) {
-            store(static_cast<T*>(a.q_out) + t * g.qo_stride + h * g.qo_head_stride);
-        } else if (hk < kv_heads) {
-            if (a.k_out != nullptr) {
-                store(static_cast<T*>(a.k_out) + t * g.ko_stride + hk * g.ko_head_stride);
-            }
-            if (a.k_cache != nullptr && k_at >= 0) {
-                store(static_cast<T*>(a.k_cache) + k_at + hk * g.kc_head_stride);
-            }
-        } else if (v_at >= 0) {
-            store(static_cast<T*>(a.v_cache) + v_at + (hk - kv_heads) * g.vc_head_stride);
+        }
+        if (cache != nullptr) {
+            T* row = cache + h * cache_head;
+            *reinterpret_cast<P*>(row + e0) = x0;
+            *reinterpret_cast<P*>(row + e1) = x1;
         }
         x0 = n0;
         x1 = n1;
@@ -164,22 +171,25 @@ __global__ void __launch_bounds__(kRopeThreads, 4)
 template <typename T, int V, bool kPairs, bool kOneAxis>
 void launch_rope_as(nb2_device* dev, const RopeArgs& a) {
     const nb2_rope_geom& g = a.g;
-    const int64_t heads = g.q_heads + g.kv_heads + (a.v != nullptr ? g.kv_heads : 0);
     const int lanes = static_cast<int>(g.rot_dim / 2 / V + (g.head_dim - g.rot_dim) / 2 / V);
-    // Heads of one thread: one while the tokens do not fill the GPU (latency
-    // counts), else kWalk (the table's rows are then read 1/kWalk as often).
-    const int64_t fill = static_cast<int64_t>(dev->num_sms) * 1024;
-    const int walk = g.tokens * heads * lanes >= kWalk * fill ? kWalk : 1;
-    int groups = static_cast<int>((heads + walk - 1) / walk);
-    groups = std::min(groups, std::max(1, kRopeThreads / lanes));
-    const int work = lanes * groups;
-    const int per = std::max(1, kRopeThreads / work);
-    const int64_t grid = (g.tokens + per - 1) / per;
+    const int64_t heads = g.q_heads + g.kv_heads + (a.v != nullptr ? g.kv_heads : 0);
+    // one head a thread while the tokens do not fill the GPU (latency counts)
+    constexpr int kWalk = walk_of(sizeof(T));
+    const int walk = g.tokens * heads * lanes >= kWalk * static_cast<int64_t>(dev->num_sms) * 1024 ? kWalk : 1;
+    auto spread = [&](int64_t n) {
+        Spread s{};
+        s.heads = static_cast<int>(n);
+        s.groups = std::min((s.heads + walk - 1) / walk, std::max(1, kRopeThreads / lanes));
+        s.tokens = std::max(1, kRopeThreads / (lanes * s.groups));
+        s.ctas = (g.tokens + s.tokens - 1) / s.tokens;
+        return s;
+    };
+    const Spread sq = spread(g.q_heads), sk = spread(g.kv_heads);
+    const int64_t grid = sq.ctas + sk.ctas * (a.v != nullptr ? 2 : 1);
     if (grid > 0x7fffffffLL) {
-        fail(kStatusUnsupported, "rope: too many tokens");
+        fail(kStatusUnsupported, "RopeAppend: too many tokens");
     }
-    rope_kernel<T, V, kPairs, kOneAxis>
-        <<<static_cast<unsigned>(grid), (work * per + 31) / 32 * 32, 0, dev->stream>>>(a, lanes, groups, per);
+    rope_kernel<T, V, kPairs, kOneAxis><<<static_cast<unsigned>(grid), kRopeThreads, 0, dev->stream>>>(a, lanes, sq, sk);
     check_cuda(cudaGetLastError(), "rope launch");
 }
 
