@@ -133,6 +133,9 @@ int nb2_tree_attention(nb2_device* dev, const nb2_tree_attn_geom* g, const void*
         if (g->head_dim > 256) {
             fail(kStatusUnsupported, "TreeAttention: at most 256 elements a head");
         }
+        if (g->tokens * (g->q_heads / g->kv_heads) > kMaxI32 - 1024) {
+            fail(kStatusUnsupported, "TreeAttention: at most 2^31 - 1025 rows a key/value head");
+        }
         need(g->max_new >= 0 && g->max_new <= kMaxI32, "TreeAttention: bad bound of new tokens");
         need(g->block_size > 0 && g->block_size <= kMaxI32 && in_i32(g->num_blocks), "TreeAttention: bad cache extents");
         need(in_i32(g->table_blocks) && g->table_stride >= g->table_blocks, "TreeAttention: bad block table extents");

@@ -38,7 +38,8 @@ __device__ __forceinline__ Request request_at(const TreeAttnArgs& a, int r, int 
     if (q.n == 0) {
         return q;
     }
-    q.bad = total < q.n || total > a.g.table_blocks * a.g.block_size || q.n > a.g.max_new;
+    constexpr int64_t kMostPlaces = 0x7fffff00; // a tile past the end still counts in 32 bits
+    q.bad = total < q.n || total > kMostPlaces || total > a.g.table_blocks * a.g.block_size || q.n > a.g.max_new;
     q.total = q.bad ? 0 : static_cast<int>(total);
     q.row_blocks = static_cast<int>((static_cast<int64_t>(q.n) * group + RT - 1) / RT);
     q.tiles = max(1, (q.total + KT - 1) / KT);

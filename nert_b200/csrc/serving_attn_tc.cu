@@ -273,65 +273,65 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (warp >= 8) {
         regs_down<88>();
         if (warp == 8) {
-        // ---- TMA: a lane a box
-        uint32_t n = 0; // tiles so far
-        const int size = static_cast<int>(g.block_size), boxes = kTile / args.box;
-        items([&](int r, const Request& rq, int64_t, int kvh, int, int t0, int t1) {
-            const int32_t* table = a.table + r * g.table_stride;
-            for (int t = t0; t < t1; ++t, ++n) {
-                const int st = n % NS;
-                const uint32_t phase = (n / NS + 1) & 1;
-                // 128 places are at most 16 boxes of a slab; lane = box + 16 * slab
-                const int box = lane & 15, slab = lane >> 4;
-                const bool mine = box < boxes && slab < S::kSlabs;
-                const int j = t * kTile + box * args.box;
-                int block = -1; // out of range: zeros
-                if (mine && j < rq.total) {
-                    block = table[j / size];
-                    block = block < 0 || block >= g.num_blocks ? -1 : block;
+            // ---- TMA: a lane a box
+            uint32_t n = 0; // tiles so far
+            const int size = static_cast<int>(g.block_size), boxes = kTile / args.box;
+            items([&](int r, const Request& rq, int64_t, int kvh, int, int t0, int t1) {
+                const int32_t* table = a.table + r * g.table_stride;
+                for (int t = t0; t < t1; ++t, ++n) {
+                    const int st = n % NS;
+                    const uint32_t phase = (n / NS + 1) & 1;
+                    // 128 places are at most 16 boxes of a slab; lane = box + 16 * slab
+                    const int box = lane & 15, slab = lane >> 4;
+                    const bool mine = box < boxes && slab < S::kSlabs;
+                    const int j = t * kTile + box * args.box;
+                    int block = -1; // out of range: zeros
+                    if (mine && j < rq.total) {
+                        block = table[j / size];
+                        block = block < 0 || block >= g.num_blocks ? -1 : block;
+                    }
+                    bool ok = mbar_wait(&k_empty[st], phase, abort_flag, a.err, args.bound);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (ok) {
+                        if (lane == 0) {
+                            mbar_arrive_expect_tx(&k_full[st], S::kKV);
+                        }
+                        __syncwarp();
+                        if (mine) {
+                            tma_load_page(ks + st * S::kKV + slab * S::kSlab + box * args.box * 128, &k_map, slab * 64, kvh,
+                                          j % size, block, &k_full[st]);
+                        }
+                    }
+                    ok = mbar_wait(&v_empty[st], phase, abort_flag, a.err, args.bound);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (ok) {
+                        if (lane == 0) {
+                            mbar_arrive_expect_tx(&v_full[st], S::kKV);
+                        }
+                        __syncwarp();
+                        if (mine) {
+                            tma_load_page(vs + st * S::kKV + slab * S::kSlab + box * args.box * 128, &v_map, slab * 64, kvh,
+                                          j % size, block, &v_full[st]);
+                        }
+                    }
                 }
-                bool ok = mbar_wait(&k_empty[st], phase, abort_flag, a.err, args.bound);
-                ok = __all_sync(0xffffffffu, ok);
-                if (ok) {
-                    if (lane == 0) {
-                        mbar_arrive_expect_tx(&k_full[st], S::kKV);
-                    }
-                    __syncwarp();
-                    if (mine) {
-                        tma_load_page(ks + st * S::kKV + slab * S::kSlab + box * args.box * 128, &k_map, slab * 64, kvh,
-                                      j % size, block, &k_full[st]);
-                    }
+            });
+            // copies in flight land before the CTA may go: their barriers complete on their own
+            for (uint32_t i = n > NS ? n - NS : 0; i < n; ++i) {
+                const long long c0 = clock64();
+                while (!mbar_try_wait(&k_full[i % NS], (i / NS) & 1) && clock64() - c0 < kWaitBoundCycles && !*abort_flag) {
                 }
-                ok = mbar_wait(&v_empty[st], phase, abort_flag, a.err, args.bound);
-                ok = __all_sync(0xffffffffu, ok);
-                if (ok) {
-                    if (lane == 0) {
-                        mbar_arrive_expect_tx(&v_full[st], S::kKV);
-                    }
-                    __syncwarp();
-                    if (mine) {
-                        tma_load_page(vs + st * S::kKV + slab * S::kSlab + box * args.box * 128, &v_map, slab * 64, kvh,
-                                      j % size, block, &v_full[st]);
-                    }
+                while (!mbar_try_wait(&v_full[i % NS], (i / NS) & 1) && clock64() - c0 < kWaitBoundCycles && !*abort_flag) {
                 }
             }
-        });
-        // copies in flight land before the CTA may go: their barriers complete on their own
-        for (uint32_t i = n > NS ? n - NS : 0; i < n; ++i) {
-            const long long c0 = clock64();
-            while (!mbar_try_wait(&k_full[i % NS], (i / NS) & 1) && clock64() - c0 < kWaitBoundCycles && !*abort_flag) {
+            if (*abort_flag) { // some barriers will not complete: give the copies the time they take
+                const long long c0 = clock64();
+                while (clock64() - c0 < 2000000) {
+                }
             }
-            while (!mbar_try_wait(&v_full[i % NS], (i / NS) & 1) && clock64() - c0 < kWaitBoundCycles && !*abort_flag) {
-            }
-        }
-        if (*abort_flag) { // some barriers will not complete: give the copies the time they take
-            const long long c0 = clock64();
-            while (clock64() - c0 < 2000000) {
-            }
-        }
         } else if (warp < 11 && lane == 0) {
             // ---- MMA: a thread a group. An MMA holds its issuing thread about as long as it runs, so one thread for both groups left the
-            // tensor cores idle while it looked for the next work (attention of 8 long contexts 236 us, with two threads MEASURED).
+            // tensor cores idle while it looked for the next work (700 clocks to issue eight, 250 to 600 between).
             const int s = warp - 9;
             uint32_t n = 0, items_done = 0, uses = 0; // tiles of all items so far, items, this group's tiles
             const uint32_t idesc_s = idesc_f16(kBf16, kHalf, false), idesc_o = idesc_f16(kBf16, DP, true);

@@ -439,6 +439,45 @@ def test_tree_attention_on_another_stream_and_in_a_graph(cuda):
     assert torch.equal(out, out2) and torch.equal(lse, lse2)
 
 
+def test_tree_attention_wait_that_runs_out(cuda):
+    """The many-row kernel's pipeline waits are bounded: past the bound it records a device error and ends, and the
+    next call is as before."""
+    b = Batch([700, 300], [40, 33], 8, 2, 128, 16, "bf16")
+    out, lse = b.run()
+    serving.synchronize()
+    dev, L = serving.context(), _lib.lib()
+    _lib.check(L.nb2_device_set_wait_bound(dev, 64))
+    try:
+        device_error(b.run)
+    finally:
+        _lib.check(L.nb2_device_set_wait_bound(dev, 0))
+    again, lse2 = b.run()
+    serving.synchronize()
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+    b.check(again, lse2)
+
+
+def test_tree_attention_negative_and_zero_scale(cuda):
+    for scale in (-0.1, 0.0):
+        for news in ([3, 1], [40, 33]):
+            b = Batch([70, 300], news, 8, 2, 128, 16, "bf16")
+            b.scale = scale
+            out, lse = b.run(scale=scale)
+            serving.synchronize()
+            b.check(out, lse)
+
+
+def test_tree_attention_no_requests(cuda):
+    k = torch.zeros(2, 16, 2, 64, device="cuda")
+    none = torch.zeros(0, device="cuda", dtype=torch.int32)
+    out, lse = serving.tree_attention(torch.randn(3, 4, 64, device="cuda"), k, k, none.view(0, 1), none, i32([0]), return_lse=True)
+    serving.synchronize()
+    assert (out == 0).all() and (lse == -math.inf).all()
+    p = serving.page_plan(none, none, none.view(0, 3), i32([4]), 16, 2)
+    serving.synchronize()
+    assert p.token_offsets.tolist() == [0] and p.slots.tolist() == [-1, -1] and p.free_head.tolist() == [0]
+
+
 def test_tree_attention_errors(cuda):
     b = Batch([20, 30], [2, 3], 4, 2, 64, 16, "bf16")
     q, table, total, off = b.q, i32(b.table), i32(b.total), i32(b.off)
