@@ -6,7 +6,7 @@
 // sum of a on; new token i sits at place l + i. The work is a few bytes a
 // token, so latency is what it costs: the prefix sums are not handed from one
 // CTA to the next. Every CTA of the token part sums all lengths itself
-// (two 4-byte words a request, read from L2) and then places its own 1,024
+// (two 4-byte words a request, read from L2) and then places its own 512
 // tokens by binary search in the sums; every CTA of the tree part handles one
 // request and sums the lengths before it.
 // Ancestors by pointer doubling: after round k a token's mask holds its 2^k
@@ -20,12 +20,17 @@ namespace nb2 {
 namespace {
 
 constexpr int kPlanThreads = 256;
-constexpr int kPlanTokens = 1024; // tokens placed by one CTA of the token part
+constexpr int kPlanTokens = 512; // tokens placed by one CTA of the token part (2,048: a step of 129 trees 16 us, 512: 10)
 constexpr int kTreeRows = kPlanMaxWords * 32 / kPlanThreads;
 
 struct ReqLens {
     int64_t old, fresh, have, want; // tokens cached / added; blocks before / after
 };
+
+// ceil(n / s) of values below 2^31, in 32 bits (a 64-bit division is a routine of a hundred instructions)
+__device__ __forceinline__ int64_t blocks_of(int64_t n, int64_t s) {
+    return (static_cast<uint32_t>(n) + static_cast<uint32_t>(s) - 1u) / static_cast<uint32_t>(s);
+}
 
 // Lengths of request r, negative ones and a sum past int32 taken as nothing.
 __device__ __forceinline__ ReqLens lens_of(const PagePlanArgs& a, int r, bool& bad) {
@@ -37,9 +42,8 @@ __device__ __forceinline__ ReqLens lens_of(const PagePlanArgs& a, int r, bool& b
         x.old = x.old < 0 ? 0 : x.old;
         x.fresh = 0;
     }
-    const int64_t s = a.g.block_size;
-    x.have = (x.old + s - 1) / s;
-    x.want = (x.old + x.fresh + s - 1) / s;
+    x.have = blocks_of(x.old, a.g.block_size);
+    x.want = blocks_of(x.old + x.fresh, a.g.block_size);
     return x;
 }
 
@@ -149,17 +153,18 @@ __device__ void token_part(const PagePlanArgs& a, int part, int parts, int* smem
         }
         const int r = owner(tok, B, static_cast<int>(t));
         const ReqLens x = lens_of(a, r, bad);
-        const int64_t p = x.old + (t - tok[r]), j = p / a.g.block_size;
+        const int64_t p = x.old + (t - tok[r]);
+        const uint32_t size = static_cast<uint32_t>(a.g.block_size), j = static_cast<uint32_t>(p) / size;
         int64_t block = -1;
         if (j < a.g.table_blocks) {
             if (j < x.have) {
                 block = a.table[r * a.g.table_stride + j];
             } else { // taken in this launch, maybe by another CTA: read it at its source
-                const int64_t f = head + blk[r] + (j - x.have);
+                const int64_t f = head + blk[r] + (static_cast<int64_t>(j) - x.have);
                 block = f >= 0 && f < a.g.free_blocks ? a.free_blocks[f] : -1;
             }
         }
-        int64_t slot = block * a.g.block_size + p % a.g.block_size;
+        int64_t slot = block * a.g.block_size + (static_cast<uint32_t>(p) - j * size);
         if (block < 0 || slot > 0x7fffffffLL) {
             slot = -1;
             short_list = true;
