@@ -404,6 +404,22 @@ def test_tree_attention_strides_padding_and_bound(cuda):
     assert (dst[:, 0] == 7).all() and (dst[:, 5] == 7).all() and (dst[:, :, :8] == 7).all()
 
 
+@pytest.mark.parametrize("news,hq,hkv", [([70, 3], 4, 2), ([90, 130], 4, 1)])
+@pytest.mark.parametrize("block", [8, 32, 256])
+@pytest.mark.parametrize("pads", [(8, 8), (64, 64), (64, 192), (0, 72), (128, 0)])
+def test_tree_attention_heads_inside_wider_ones(cuda, news, hq, hkv, block, pads):
+    """Keys and values of many rows whose heads lie in wider ones, each its own, at any multiple of 16 bytes."""
+    b = Batch([200, 77], news, hq, hkv, 128, block, "bf16")
+    for name, pad in zip(("kc", "vc"), pads):
+        x = getattr(b, name)
+        wide = torch.full((*x.shape[:3], 128 + pad), float("nan"), device="cuda", dtype=x.dtype)
+        wide[..., :128] = x
+        setattr(b, name, wide[..., :128])
+    out, lse = b.run()
+    serving.synchronize()
+    b.check(out, lse)
+
+
 def test_tree_attention_offsets_past_32_bits(cuda):
     """Blocks more than 2^31 elements apart."""
     b = Batch([100], [9], 4, 1, 64, 64, "bf16")
