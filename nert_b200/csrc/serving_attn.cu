@@ -124,9 +124,9 @@ struct Shape {
 };
 
 template <typename T, int DP, int WR, int WK>
-__global__ void __launch_bounds__(32 * WR * WK, Shape<T, DP, WR, WK>::kPerSm) tree_attn_kernel(const __grid_constant__ TreeAttnArgs a, int group,
-                                                                 int sms, float* part_o, float2* part_ml,
-                                                                 uint32_t* tickets) {
+__global__ void __launch_bounds__(32 * WR * WK, Shape<T, DP, WR, WK>::kPerSm)
+    tree_attn_kernel(const __grid_constant__ TreeAttnArgs a, int group, int sms, float* part_o, float2* part_ml,
+                     uint32_t* tickets) {
     using S = Shape<T, DP, WR, WK>;
     constexpr int NT = S::kThreads, RT = S::RT, KT = S::KT, KW = S::KW, NS = S::NS;
     constexpr int NB = KW / 8; // 8-place column blocks of a warp's scores

@@ -66,7 +66,8 @@ __device__ __forceinline__ void walk_list(const int32_t* ids, int lo, int hi, in
 
 // kLevel: every row starts on a whole pack, in the logits and in the results.
 template <typename TI, typename TO, bool kBias, bool kLevel>
-__global__ void __launch_bounds__(kLogitThreads, kLevel ? 5 : 1) logits_kernel(const __grid_constant__ LogitsArgs a, int rows_per_cta) {
+__global__ void __launch_bounds__(kLogitThreads, kLevel ? 5 : 1)
+    logits_kernel(const __grid_constant__ LogitsArgs a, int rows_per_cta) {
     extern __shared__ uint32_t logit_smem[];
     // logits of a thread and step: the wider side is 16 bytes, so that a warp's loads and stores have no gaps
     constexpr int V = 16 / (sizeof(TI) > sizeof(TO) ? sizeof(TI) : sizeof(TO));
