@@ -16,7 +16,7 @@
 // CTA reads the same number of tiles whatever the lengths. An item inside one span is finished by
 // its CTA; of one that is cut, each CTA leaves (O, m, sum) in its own slot (a span cuts at most its
 // first and its last item: two slots a CTA) and the CTA that arrives last adds the pieces in span
-// order, so the result does not depend on which one that is.
+// order, so the result does not depend on which one that is (where pieces are many, a second launch adds them in the same order).
 //
 // Within a CTA, WR x WK warps: row group x part of the tile's places. The warps of a row group run
 // the softmax on their own places and join at the end of the item. Tiles come by 16-byte cp.async
@@ -593,7 +593,7 @@ __global__ void __launch_bounds__(32 * WR * WK, Shape<T, DP, WR, WK>::kPerSm)
                 }
             }
         }
-        if (!whole) {
+        if (!whole && tickets != nullptr) { // null: a launch of its own joins
             const int c0 = cta_of(item_w0, W, grid), c1 = cta_of(item_w1 - 1, W, grid);
             __threadfence();
             __syncthreads();
@@ -632,10 +632,19 @@ void launch_attn(nb2_device* dev, const TreeAttnArgs& a) {
     const int grid = dev->num_sms * per_sm[dev->ordinal];
     const size_t o_bytes = static_cast<size_t>(grid) * 2 * S::RT * DP * 4;
     uint8_t* ws = static_cast<uint8_t*>(dev->scratch(o_bytes + static_cast<size_t>(grid) * 2 * S::RT * 8));
-    kernel<<<grid, S::kThreads, S::kSmem, dev->stream>>>(a, static_cast<int>(a.g.q_heads / a.g.kv_heads), dev->num_sms,
-                                                         reinterpret_cast<float*>(ws),
-                                                         reinterpret_cast<float2*>(ws + o_bytes), dev->tickets(grid));
+    const int group = static_cast<int>(a.g.q_heads / a.g.kv_heads);
+    float* part_o = reinterpret_cast<float*>(ws);
+    float2* part_ml = reinterpret_cast<float2*>(ws + o_bytes);
+    dim3 join;
+    const bool apart = join_apart(a, grid, S::RT, DP, join);
+    kernel<<<grid, S::kThreads, S::kSmem, dev->stream>>>(a, group, dev->num_sms, part_o, part_ml,
+                                                         apart ? nullptr : dev->tickets(grid));
     check_cuda(cudaGetLastError(), "tree attention launch");
+    if (apart) {
+        join_kernel<T, DP, S::RT, S::KT, false>
+            <<<join, kJoinThreads, 0, dev->stream>>>(a, group, grid, dev->num_sms, part_o, part_ml);
+    }
+    check_cuda(cudaGetLastError(), "tree attention join");
 }
 
 template <typename T, int DP>

@@ -4,6 +4,8 @@
 
 #include "serving.cuh"
 
+#include <algorithm>
+
 namespace nb2 {
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -118,11 +120,25 @@ __device__ __forceinline__ void store_row4(const TreeAttnArgs& a, int64_t first,
 // The pieces of an item in the slots of CTAs c0 .. c1 (the first left its piece in its second slot,
 // the others theirs in their first), added in that order and stored; NT threads. A thread takes kElems groups of
 // four elements through kPieces pieces at a time, all their loads in flight: one after another the loads of a short
-// item's pieces (up to one a tile) took longer than its tiles.
-template <typename T, int DP, int RT, int NT, int kElems, int kPieces>
+// item's pieces (up to one a tile) took longer than its tiles. kColumns: pieces lie four elements by four, the rows together;
+// a warp takes 8 rows x 16 elements. `step` threads share the item.
+template <typename T, int DP, int RT, int NT, int kElems, int kPieces, bool kColumns>
 __device__ __forceinline__ void join_pieces_as(const TreeAttnArgs& a, const float* part_o, const float2* part_ml, int c0,
-                                               int c1, int64_t first, int64_t kvh, int group, int rho0, int rows, int tid) {
-    for (int i0 = tid; i0 < rows * (DP / 4); i0 += kElems * NT) {
+                                               int c1, int64_t first, int64_t kvh, int group, int rho0, int rows, int tid,
+                                               int step) {
+    static_assert(!kColumns || kElems == 1, "the columns' order is that of one element a thread");
+    auto place = [](int i, int& row, int& d) {
+        if constexpr (kColumns) {
+            const int r = i >> 5;
+            row = r / (DP / 16) * 8 + ((i >> 2) & 7);
+            d = r % (DP / 16) * 16 + (i & 3) * 4;
+        } else {
+            row = i / (DP / 4);
+            d = (i - row * (DP / 4)) * 4;
+        }
+    };
+    const int all = (kColumns ? (rows + 7) / 8 * 8 : rows) * (DP / 4);
+    for (int i0 = tid; i0 < all; i0 += kElems * step) {
         float m[kElems], z[kElems];
         float4 x[kElems];
 #pragma unroll
@@ -140,11 +156,13 @@ __device__ __forceinline__ void join_pieces_as(const TreeAttnArgs& a, const floa
                 const int64_t slot = 2 * static_cast<int64_t>(c + p) + (c + p == c0 ? 1 : 0);
 #pragma unroll
                 for (int u = 0; u < kElems; ++u) {
-                    const int i = i0 + u * NT, row = i / (DP / 4), d = (i - row * (DP / 4)) * 4;
+                    int row, d;
+                    place(i0 + u * step, row, d);
                     ml[p][u] = make_float2(-INFINITY, 0.0f);
                     if (c + p <= c1 && row < rows && d < a.g.head_dim) {
                         ml[p][u] = __ldcg(&part_ml[slot * RT + row]);
-                        y[p][u] = __ldcg(reinterpret_cast<const float4*>(part_o + (slot * RT + row) * DP + d));
+                        y[p][u] = __ldcg(reinterpret_cast<const float4*>(
+                            part_o + (kColumns ? (slot * (DP / 4) + d / 4) * RT * 4 + row * 4 : (slot * RT + row) * DP + d)));
                     }
                 }
             }
@@ -165,7 +183,8 @@ __device__ __forceinline__ void join_pieces_as(const TreeAttnArgs& a, const floa
         }
 #pragma unroll
         for (int u = 0; u < kElems; ++u) {
-            const int i = i0 + u * NT, row = i / (DP / 4), d = (i - row * (DP / 4)) * 4;
+            int row, d;
+            place(i0 + u * step, row, d);
             if (row < rows && d < a.g.head_dim) {
                 store_row4<T>(a, first, kvh, group, rho0 + row, d, x[u], m[u], z[u]);
             }
@@ -177,9 +196,9 @@ template <typename T, int DP, int RT, int NT>
 __device__ __forceinline__ void join_pieces(const TreeAttnArgs& a, const float* part_o, const float2* part_ml, int c0, int c1,
                                             int64_t first, int64_t kvh, int group, int rho0, int rows, int tid) {
     if (rows * (DP / 4) <= 2 * NT) {
-        join_pieces_as<T, DP, RT, NT, 1, 8>(a, part_o, part_ml, c0, c1, first, kvh, group, rho0, rows, tid);
+        join_pieces_as<T, DP, RT, NT, 1, 8, false>(a, part_o, part_ml, c0, c1, first, kvh, group, rho0, rows, tid, NT);
     } else {
-        join_pieces_as<T, DP, RT, NT, 4, 2>(a, part_o, part_ml, c0, c1, first, kvh, group, rho0, rows, tid);
+        join_pieces_as<T, DP, RT, NT, 4, 2, false>(a, part_o, part_ml, c0, c1, first, kvh, group, rho0, rows, tid, NT);
     }
 }
 
@@ -209,12 +228,16 @@ __device__ __forceinline__ void spare_tokens(const TreeAttnArgs& a, int tid, int
 constexpr int kMinSpan = 4;
 
 // This CTA's span of the W units, and the request that its first unit is in. All NT threads.
+__device__ __forceinline__ int64_t span_count(int64_t W, int64_t ctas, int least) { // none is empty
+    return min(ctas, max(W / kMinSpan, min(W, static_cast<int64_t>(least))));
+}
+
 struct Span {
     int64_t W, grid, w0, w1;
     int request;          // holds unit w0
     int64_t request_unit; // first unit of that request
     __device__ __forceinline__ void set(int64_t cta, int least) {
-        grid = min(static_cast<int64_t>(gridDim.x), max(W / kMinSpan, min(W, static_cast<int64_t>(least)))); // none is empty
+        grid = span_count(W, gridDim.x, least);
         w0 = cta < grid ? cta * W / grid : 0;
         w1 = cta < grid ? (cta + 1) * W / grid : 0;
     }
@@ -290,6 +313,76 @@ __device__ __forceinline__ Span find_span(const TreeAttnArgs& a, int group, int 
     s.request = static_cast<int>(found[0]);
     s.request_unit = found[1];
     return s;
+}
+
+// ---- the join of few items, by a launch of its own ----------------------------------
+
+// An item's pieces are joined by one CTA when it has a few; where few items share the GPU (one long context), each is in
+// many, which that CTA reads one after another while the others are gone: then a second launch joins them, a slice
+// of an item's elements a CTA. By the CTA / by the launch, bfloat16, 60,000 places: 64 tokens, 32/8 heads of 128 (18 pieces
+// of 128 KB) 119 / 99 us, 8/1 heads (74 pieces) 154 / 58; 8 tokens, 32/8 heads (18 of 16 KB) 96 / 93; 8,000 places, 33 tokens 66 / 40.
+// One token (37 of 2 KB) takes 59 us and 57 with no join at all, so nothing would be gained there.
+constexpr int kJoinThreads = 256;
+constexpr int64_t kJoinApart = 256 << 10; // bytes of an item's pieces from which on that is faster
+
+inline bool join_apart(const TreeAttnArgs& a, int ctas, int RT, int DP, dim3& grid) {
+    const nb2_tree_attn_geom& g = a.g;
+    const int64_t rows = std::min(g.max_new, g.tokens) * (g.q_heads / g.kv_heads);
+    const int64_t items = g.batch * g.kv_heads * ((rows + RT - 1) / RT), most = (std::min<int64_t>(rows, RT) + 7) / 8 * 8;
+    grid = dim3(static_cast<unsigned>((most * (DP / 4) + kJoinThreads - 1) / kJoinThreads), static_cast<unsigned>(items));
+    return items > 0 && g.batch <= kJoinThreads && items <= 65535 && most * DP * 4 * ctas > kJoinApart * items;
+}
+
+template <typename T, int DP, int RT, int KT, bool kColumns>
+__global__ void __launch_bounds__(kJoinThreads)
+    join_kernel(const __grid_constant__ TreeAttnArgs a, int group, int ctas, int least, const float* part_o,
+                const float2* part_ml) {
+    __shared__ int64_t warp_items[kJoinThreads / 32], warp_units[kJoinThreads / 32], found[3];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t kv_heads = a.g.kv_heads, wanted = blockIdx.y;
+    Request q{};
+    if (tid < a.g.batch) {
+        q = request_at<RT, KT>(a, tid, group);
+    }
+    const int64_t items = q.row_blocks * kv_heads, units = q.units(kv_heads);
+    int64_t items_to = items, units_to = units, W = 0, all = 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, items_to, o), y = __shfl_up_sync(0xffffffffu, units_to, o);
+        items_to += lane >= o ? x : 0;
+        units_to += lane >= o ? y : 0;
+    }
+    if (lane == 31) {
+        warp_items[warp] = items_to;
+        warp_units[warp] = units_to;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kJoinThreads / 32; ++w) {
+        items_to += w < warp ? warp_items[w] : 0;
+        units_to += w < warp ? warp_units[w] : 0;
+        all += warp_items[w];
+        W += warp_units[w];
+    }
+    if (items_to - items <= wanted && wanted < items_to) {
+        found[0] = tid;
+        found[1] = wanted - (items_to - items);
+        found[2] = units_to - units;
+    }
+    __syncthreads();
+    if (wanted >= all) {
+        return;
+    }
+    const Request rq = request_at<RT, KT>(a, static_cast<int>(found[0]), group);
+    const int64_t item = found[1], w0 = found[2] + item * rq.per_item() + rq.extra, n = span_count(W, ctas, least);
+    const int64_t kvh = item / rq.row_blocks;
+    const int rb = static_cast<int>(item - kvh * rq.row_blocks), rows = min(RT, rq.n * group - rb * RT);
+    const int c0 = cta_of(w0, W, n), c1 = cta_of(w0 + rq.tiles - 1, W, n);
+    if (c0 < c1) { // otherwise one CTA had all of it, and stored it
+        join_pieces_as<T, DP, RT, kJoinThreads, 1, 8, kColumns>(a, part_o, part_ml, c0, c1, rq.first, kvh, group, rb * RT, rows,
+                                                                static_cast<int>(blockIdx.x) * kJoinThreads + tid,
+                                                                static_cast<int>(gridDim.x) * kJoinThreads);
+    }
 }
 
 // The tensor-core kernel for many rows (serving_attn_tc.cu): whether it takes the call, and the call.

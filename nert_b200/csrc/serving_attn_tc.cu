@@ -805,6 +805,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (live && (kTiles == 2 || s == 0)) {
                     __stcg(args.part_ml + slot * RT + row, make_float2(mm, zs));
                 }
+            }
+            if (!whole && args.tickets != nullptr) { // null: a launch of its own joins
                 const int p0 = cta_of(item_w0, span.W, span.grid), p1 = cta_of(item_w0 + rq.tiles - 1, span.W, span.grid);
                 __threadfence();
                 bar_named(1, kSoftmax);
@@ -917,10 +919,18 @@ void launch_tc(nb2_device* dev, const TreeAttnArgs& a) {
     const int grid = dev->num_sms;
     const size_t o_bytes = static_cast<size_t>(grid) * 2 * S::RT * DP * 4;
     uint8_t* ws = static_cast<uint8_t*>(dev->scratch(o_bytes + static_cast<size_t>(grid) * 2 * S::RT * 8));
-    TcArgs args{a, static_cast<int>(g.q_heads / g.kv_heads), box, reinterpret_cast<float*>(ws),
-                reinterpret_cast<float2*>(ws + o_bytes), dev->tickets(grid), dev->wait_bound};
+    const int group = static_cast<int>(g.q_heads / g.kv_heads);
+    float* part_o = reinterpret_cast<float*>(ws);
+    float2* part_ml = reinterpret_cast<float2*>(ws + o_bytes);
+    dim3 join;
+    const bool apart = join_apart(a, grid, S::RT, DP, join);
+    const TcArgs args{a, group, box, part_o, part_ml, apart ? nullptr : dev->tickets(grid), dev->wait_bound};
     kernel<<<grid, kTcThreads, S::kSmem, dev->stream>>>(args, km, vm);
     check_cuda(cudaGetLastError(), "tree attention launch");
+    if (apart) {
+        join_kernel<T, DP, S::RT, kTile, true><<<join, kJoinThreads, 0, dev->stream>>>(a, group, grid, 1, part_o, part_ml);
+    }
+    check_cuda(cudaGetLastError(), "tree attention join");
 }
 
 template <typename T, int DP>

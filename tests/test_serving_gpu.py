@@ -404,6 +404,22 @@ def test_tree_attention_strides_padding_and_bound(cuda):
     assert (dst[:, 0] == 7).all() and (dst[:, 5] == 7).all() and (dst[:, :, :8] == 7).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("olds,news,hq,hkv,dim,block", [
+    ([40000], [3], 4, 1, 64, 16), ([30000], [12], 4, 1, 128, 16), ([30000, 0], [33, 2], 8, 1, 128, 64), ([9000], [70], 6, 3, 96, 32),
+    ([12000, 7, 5000], [130, 0, 1], 2, 1, 64, 16), ([700 + 37 * i for i in range(24)], [40 - i for i in range(24)], 32, 8, 128, 16),
+    ([400 + 91 * i for i in range(40)], [1 + i % 3 for i in range(40)], 16, 4, 64, 16), ([8000], [5], 3, 1, 256, 16),
+])
+def test_tree_attention_pieces(cuda, dtype, olds, news, hq, hkv, dim, block):
+    """A few items in many pieces each, and many items in a few: two calls agree in every bit."""
+    b = Batch(olds, news, hq, hkv, dim, block, dtype, seed=3)
+    out, lse = b.run()
+    again, lse2 = b.run()
+    serving.synchronize()
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+    b.check(out, lse)
+
+
 @pytest.mark.parametrize("news,hq,hkv", [([70, 3], 4, 2), ([90, 130], 4, 1)])
 @pytest.mark.parametrize("block", [8, 32, 256])
 @pytest.mark.parametrize("pads", [(8, 8), (64, 64), (64, 192), (0, 72), (128, 0)])
