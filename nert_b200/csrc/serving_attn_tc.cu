@@ -28,7 +28,8 @@
 // memory before its P is released, and adds p * v itself for the rows that see the place.
 //
 // Every wait is bounded; a thread that gives up raises the CTA's abort flag, after which all loops run
-// out without waiting, touching tensor memory or storing results.
+// out without waiting: no product or copy is issued any more and no result is stored (the softmax threads
+// still read and write their own tensor memory, which is held until the CTA ends).
 
 #include "serving_attn.cuh"
 
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     uint8_t* ks = qs + S::kQ;
     uint8_t* vs = ks + NS * S::kKV;
     __shared__ uint64_t k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], s_full[2][2], p_full[2][2], o_done[2][2], q_full,
-        drain;
+        q_taken, drain;
     __shared__ int64_t red[kTcThreads / 32], found[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word, is_last, hole_word;
@@ -231,6 +232,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
         }
         mbar_init(&q_full, kSoftmax);
+        mbar_init(&q_taken, 2);
         mbar_init(&drain, 2);
         abort_word = 0;
         hole_word = 0;
@@ -352,6 +354,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             items([&](int, const Request&, int64_t, int, int, int t0, int t1) {
                 bool ok = wait(&q_full, items_done & 1);
                 ++items_done;
+                mbar_arrive(&q_taken);
                 constexpr int kStep = kTiles == 2 ? 1 : 2;
                 const int i0 = kTiles == 2 ? 0 : s, nt = t1 - t0;
                 // S = Q K^T of half h of a tile; the last half's commit gives K back
@@ -418,7 +421,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const bool flip = g.scale < 0.0f; // Q is negated instead, so that a row's largest product is its maximum
         const int size = static_cast<int>(g.block_size);
         const int share = kTiles == 2 ? kSoftmax : kTile; // threads that prepare a tile together
-        uint32_t s_uses = 0, n = 0;
+        uint32_t s_uses = 0, n = 0, items_begun = 0;
         uint32_t zeros[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
@@ -488,12 +491,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 });
             }
             fence_proxy_async_smem();
+            // Not before both MMA threads have seen the item before: one that has no tile of it is awaited by nothing else, and
+            // two items behind it would take this one's phase for one that is still to come.
+            bool ok = items_begun == 0 || mbar_wait(&q_taken, (items_begun - 1) & 1, abort_flag, a.err, args.bound);
+            ++items_begun;
             mbar_arrive(&q_full);
             bar_named(1, kSoftmax);
             const bool holes = *const_cast<volatile int*>(&hole_word) != 0;
 
             float m = -INFINITY, z = 0.0f; // reference and sum of this row
-            bool ok = !*abort_flag;
+            ok = ok && !*abort_flag;
             uint32_t halves = 0; // of this item, whose weights this thread has given
             // After the product of the last weights that this thread has given. (A barrier for each half: the phase before the one
             // awaited is then always over, its half's next scores having been made after it.)

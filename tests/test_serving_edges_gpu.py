@@ -1,0 +1,28 @@
+"""The serving rows on the GPU where calls meet an edge: items of a single tile,
+requests out of their bounds beside good ones, batches next to a launch limit,
+replayed graphs, other GPUs and threads, views with odd strides. The plain
+implementations and tolerances are those of test_serving_gpu."""
+
+import numpy as np
+import pytest
+
+from nert_b200 import serving
+from test_serving_gpu import Batch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("news", [(33, 40), (33, 64)])
+def test_tree_attention_many_items_of_one_tile(cuda, dim, news):
+    """Items of one tile of places one after another in a CTA: half of the many-row kernel has nothing to do in them."""
+    rng = np.random.default_rng(5)
+    new = rng.integers(news[0], news[1] + 1, 300)
+    b = Batch(rng.integers(0, 64, 300), new, 4, 2, dim, 16, "bf16", seed=dim)
+    out, lse = b.run()
+    for _ in range(5):
+        again, lse2 = b.run()
+    serving.synchronize()
+    assert np.array_equal(out.float().cpu().numpy(), again.float().cpu().numpy())
+    assert np.array_equal(lse.cpu().numpy(), lse2.cpu().numpy())
+    b.check(out, lse)
