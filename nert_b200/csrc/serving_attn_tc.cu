@@ -187,6 +187,10 @@ struct TcShape {
     static constexpr int kKV = kSlabs * kSlab;        // a K or a V tile
     static constexpr int kQ = kTiles * kKV;
     static constexpr int NS = DP == 64 ? 4 : kTiles == 2 ? 2 : 3;
+    // Barriers of landed tiles, taken in turn. A wait by parity is right only where the barrier's phase before is known to be
+    // over, and a group knows that of its own tiles: with alternate tiles a group and an odd ring, a stage's
+    // tile before is the other group's, so that there are barriers for two rounds of the ring.
+    static constexpr int NF = kTiles == 1 && NS % 2 == 1 ? 2 * NS : NS;
     static constexpr int kSmem = 1024 + kQ + 2 * NS * kKV;
 };
 
@@ -195,7 +199,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     tree_attn_tc_kernel(const __grid_constant__ TcArgs args, const __grid_constant__ CUtensorMap k_map,
                         const __grid_constant__ CUtensorMap v_map) {
     using S = TcShape<DP, kTiles>;
-    constexpr int NS = S::NS, RT = S::RT;
+    constexpr int NS = S::NS, NF = S::NF, RT = S::RT;
     constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
     const TreeAttnArgs& a = args.a;
     const nb2_tree_attn_geom& g = a.g;
@@ -203,7 +207,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tc_dyn) + 1023) & ~uintptr_t(1023));
     uint8_t* ks = qs + S::kQ;
     uint8_t* vs = ks + NS * S::kKV;
-    __shared__ uint64_t k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], s_full[2][2], p_full[2][2], o_done[2][2], q_full,
+    __shared__ uint64_t k_full[NF], k_empty[NS], v_full[NF], v_empty[NS], s_full[2][2], p_full[2][2], o_done[2][2], q_full,
         q_taken, drain;
     __shared__ int64_t red[kTcThreads / 32], found[2];
     __shared__ uint32_t tmem_slot;
@@ -219,10 +223,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     bool bad = false;
     if (tid == 0) {
         for (int i = 0; i < NS; ++i) {
-            mbar_init(&k_full[i], 1);
             mbar_init(&k_empty[i], kTiles);
-            mbar_init(&v_full[i], 1);
             mbar_init(&v_empty[i], kTiles);
+        }
+        for (int i = 0; i < NF; ++i) {
+            mbar_init(&k_full[i], 1);
+            mbar_init(&v_full[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             for (int h = 0; h < 2; ++h) {
@@ -302,24 +308,24 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     ok = __all_sync(0xffffffffu, ok);
                     if (ok) {
                         if (lane == 0) {
-                            mbar_arrive_expect_tx(&k_full[st], S::kKV);
+                            mbar_arrive_expect_tx(&k_full[n % NF], S::kKV);
                         }
                         __syncwarp();
                         if (mine) {
                             tma_load_page(ks + st * S::kKV + slab * S::kSlab + box * args.box * 128, &k_map, slab * 64, kvh,
-                                          j % size, block, &k_full[st]);
+                                          j % size, block, &k_full[n % NF]);
                         }
                     }
                     ok = mbar_wait(&v_empty[st], phase, abort_flag, a.err, args.bound);
                     ok = __all_sync(0xffffffffu, ok);
                     if (ok) {
                         if (lane == 0) {
-                            mbar_arrive_expect_tx(&v_full[st], S::kKV);
+                            mbar_arrive_expect_tx(&v_full[n % NF], S::kKV);
                         }
                         __syncwarp();
                         if (mine) {
                             tma_load_page(vs + st * S::kKV + slab * S::kSlab + box * args.box * 128, &v_map, slab * 64, kvh,
-                                          j % size, block, &v_full[st]);
+                                          j % size, block, &v_full[n % NF]);
                         }
                     }
                 }
@@ -327,9 +333,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // copies in flight land before the CTA may go: their barriers complete on their own
             for (uint32_t i = n > NS ? n - NS : 0; i < n; ++i) {
                 const long long c0 = clock64();
-                while (!mbar_try_wait(&k_full[i % NS], (i / NS) & 1) && clock64() - c0 < kWaitBoundCycles && !*abort_flag) {
+                while (!mbar_try_wait(&k_full[i % NF], (i / NF) & 1) && clock64() - c0 < kWaitBoundCycles && !*abort_flag) {
                 }
-                while (!mbar_try_wait(&v_full[i % NS], (i / NS) & 1) && clock64() - c0 < kWaitBoundCycles && !*abort_flag) {
+                while (!mbar_try_wait(&v_full[i % NF], (i / NF) & 1) && clock64() - c0 < kWaitBoundCycles && !*abort_flag) {
                 }
             }
             if (*abort_flag) { // some barriers will not complete: give the copies the time they take
@@ -360,7 +366,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 // S = Q K^T of half h of a tile; the last half's commit gives K back
                 auto scores = [&](int i, int h) {
                     const uint32_t st = (n + i) % NS;
-                    ok = ok && wait(&k_full[st], ((n + i) / NS) & 1);
+                    ok = ok && wait(&k_full[(n + i) % NF], ((n + i) / NF) & 1);
                     if (ok) {
                         const uint32_t k = smem_u32(ks + st * S::kKV) + h * kHalf * 128;
 #pragma unroll
@@ -380,7 +386,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 for (int i = i0; i < nt; i += kStep, ++uses) {
                     const uint32_t st = (n + i) % NS;
-                    ok = ok && wait(&v_full[st], ((n + i) / NS) & 1);
+                    ok = ok && wait(&v_full[(n + i) % NF], ((n + i) / NF) & 1);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         // O += P V of the half, then the half's next scores where its weights were
@@ -564,7 +570,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             sees[w] = see_bits(mask, g.mask_words, tok, j0 + 32 * w - old);
                         }
                     }
-                    ok = mbar_wait(&v_full[tile % NS], (tile / NS) & 1, abort_flag, a.err, args.bound) && ok;
+                    ok = mbar_wait(&v_full[tile % NF], (tile / NF) & 1, abort_flag, a.err, args.bound) && ok;
 #pragma unroll 1
                     for (int sl = 0; sl < S::kSlabs; ++sl) {
                         if (kTiles == 2 && S::kSlabs == 2 && sl != s) {

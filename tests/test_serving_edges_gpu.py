@@ -26,3 +26,16 @@ def test_tree_attention_many_items_of_one_tile(cuda, dim, news):
     assert np.array_equal(out.float().cpu().numpy(), again.float().cpu().numpy())
     assert np.array_equal(lse.cpu().numpy(), lse2.cpu().numpy())
     b.check(out, lse)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [72, 128])
+def test_tree_attention_alternate_tiles(cuda, dtype, dim):
+    """Up to 128 rows over one to a hundred tiles: the groups take alternate tiles from a ring of three."""
+    b = Batch([5000, 0, 390, 1020, 12000, 100, 640], [100, 66, 128, 97, 70, 28, 65], 3, 3, dim, 32, dtype, seed=dim)
+    out, lse = b.run()
+    for _ in range(10):
+        again, lse2 = b.run()
+        assert (out == again).all() and (lse == lse2).all()
+    serving.synchronize()
+    b.check(out, lse)
