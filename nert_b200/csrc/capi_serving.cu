@@ -111,7 +111,8 @@ int nb2_rope_append(nb2_device* dev, const nb2_rope_geom* g, const void* q, cons
                  (k_cache != nullptr) == (slots != nullptr),
              "RopeAppend: v, slots and both caches come together");
         need(k_cache != nullptr || k_out != nullptr, "RopeAppend: the keys have nowhere to go");
-        need(k_cache == nullptr || (g->block_size > 0 && g->num_blocks >= 0), "RopeAppend: bad cache extents");
+        need(k_cache == nullptr || (g->block_size > 0 && g->block_size <= kMaxI32 && in_i32(g->num_blocks)),
+             "RopeAppend: bad cache extents");
         bind(dev);
         rope_append(dev, RopeArgs{*g, q, k, v, table, positions, slots, q_out, k_out, k_cache, v_cache, nullptr});
     });
