@@ -17,6 +17,9 @@
 
 #include "serving.cuh"
 
+#include <algorithm>
+#include <mutex>
+
 namespace nb2 {
 
 namespace {
@@ -308,13 +311,15 @@ void page_plan(nb2_device* dev, PagePlanArgs a) {
     }
     const int64_t w = a.g.mask_words;
     const size_t smem = static_cast<size_t>(std::max(2 * (a.g.batch + 1), trees > 0 ? 32 * w * (w + 1) : 0)) * 4;
-    static size_t attr_bytes[64] = {};
-    if (smem > 48 * 1024 && attr_bytes[dev->ordinal] < smem) {
+    // Asked for once a GPU, whatever this call's size: the 48 KB that need no asking hold the static part too, and a value
+    // that followed the calls could be lowered by one thread between another's request and its launch.
+    constexpr int64_t kMostSmem = 4 * std::max(2 * (kPlanMaxBatch + 1), 32 * kPlanMaxWords * (kPlanMaxWords + 1));
+    static std::once_flag asked[64];
+    std::call_once(asked[dev->ordinal], [] {
         check_cuda(cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        static_cast<int>(smem)),
+                                        static_cast<int>(kMostSmem)),
                    "cudaFuncSetAttribute(page plan)");
-        attr_bytes[dev->ordinal] = smem;
-    }
+    });
     page_plan_kernel<<<static_cast<unsigned>(parts + trees), kPlanThreads, smem, dev->stream>>>(
         a, static_cast<int>(parts));
     check_cuda(cudaGetLastError(), "page plan launch");

@@ -3,9 +3,14 @@ requests out of their bounds beside good ones, batches next to a launch limit,
 replayed graphs, other GPUs and threads, views with odd strides. The plain
 implementations and tolerances are those of test_serving_gpu."""
 
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
+from conftest import ROOT
 from nert_b200 import serving
 from test_serving_gpu import Batch
 
@@ -39,3 +44,28 @@ def test_tree_attention_alternate_tiles(cuda, dtype, dim):
         assert (out == again).all() and (lse == lse2).all()
     serving.synchronize()
     b.check(out, lse)
+
+
+PLAN_ALONE = """
+import sys
+import numpy as np, torch
+from nert_b200 import serving
+n = int(sys.argv[1])
+i32 = lambda x: torch.tensor(np.asarray(x, np.int32), device="cuda")
+new = np.arange(n) % 3
+p = serving.page_plan(i32(np.full(n, 5)), i32(new), i32(np.arange(n)[:, None]), i32([0]), 16, int(new.sum()))
+serving.synchronize()
+r = np.repeat(np.arange(n), new)
+i = np.concatenate([np.arange(x) for x in new])
+assert np.array_equal(p.slots.cpu().numpy(), 16 * r + 5 + i)
+assert np.array_equal(p.token_offsets.cpu().numpy(), np.concatenate([[0], np.cumsum(new)]))
+"""
+
+
+@pytest.mark.parametrize("batch", [6119, 6130, 6143, 6144, 8192])
+def test_page_plan_of_any_batch_as_the_first_call(cuda, batch):
+    """Around 48 KB of shared memory, static and dynamic part together: in a process of its own, where no larger
+    call has raised the kernel's limit before."""
+    done = subprocess.run([sys.executable, "-c", PLAN_ALONE, str(batch)], cwd=ROOT, capture_output=True, text=True,
+                          env=os.environ | {"PYTHONPATH": ROOT}, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
