@@ -344,7 +344,9 @@ __global__ void __launch_bounds__(kJoinThreads)
     if (tid < a.g.batch) {
         q = request_at<RT, KT>(a, tid, group);
     }
-    const int64_t items = q.row_blocks * kv_heads, units = q.units(kv_heads);
+    // A request out of its bounds may have more rows than the grid was sized for. Its items are of one tile, which is never
+    // cut, so they need no join and are not counted.
+    const int64_t items = q.bad ? 0 : q.row_blocks * kv_heads, units = q.units(kv_heads);
     int64_t items_to = items, units_to = units, W = 0, all = 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {

@@ -3,15 +3,17 @@ requests out of their bounds beside good ones, batches next to a launch limit,
 replayed graphs, other GPUs and threads, views with odd strides. The plain
 implementations and tolerances are those of test_serving_gpu."""
 
+import math
 import os
 import subprocess
 import sys
 
 import numpy as np
 import pytest
+import torch
 
 from conftest import ROOT
-from nert_b200 import serving
+from nert_b200 import _lib, serving
 from test_serving_gpu import Batch
 
 pytestmark = pytest.mark.gpu
@@ -49,7 +51,7 @@ def test_tree_attention_alternate_tiles(cuda, dtype, dim):
 PLAN_ALONE = """
 import sys
 import numpy as np, torch
-from nert_b200 import serving
+from nert_b200 import _lib, serving
 n = int(sys.argv[1])
 i32 = lambda x: torch.tensor(np.asarray(x, np.int32), device="cuda")
 new = np.arange(n) % 3
@@ -69,3 +71,32 @@ def test_page_plan_of_any_batch_as_the_first_call(cuda, batch):
     done = subprocess.run([sys.executable, "-c", PLAN_ALONE, str(batch)], cwd=ROOT, capture_output=True, text=True,
                           env=os.environ | {"PYTHONPATH": ROOT}, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("dtype,dim,news,hq,hkv", [
+    ("f32", 128, [200, 64, 40], 4, 1),  # joined by the mma.sync kernel's second launch, blocks of 64 rows
+    ("bf16", 128, [200, 64, 64], 8, 1),  # by the tcgen05 kernel's, blocks of 256 rows
+    ("f16", 64, [400, 90, 1], 1, 1),  # blocks of 128 rows
+])
+@pytest.mark.parametrize("first", [True, False])
+def test_tree_attention_request_past_its_bound_beside_good_ones(cuda, dtype, dim, news, hq, hkv, first):
+    """Only the request with more new tokens than max_new is refused: it gets out 0 and a device error, and those
+    after it, split over many CTAs, what they get without it."""
+    olds, most = [0, 30000, 20000], news[1]
+    if not first:
+        olds, news = olds[1:] + olds[:1], news[1:] + news[:1]
+    b = Batch(olds, news, hq, hkv, dim, 16, dtype, seed=4)
+    out = torch.full_like(b.q, 7.0)
+    _, lse = b.run(max_new=most, out=out)
+    with pytest.raises(_lib.NB2Error) as e:
+        serving.synchronize()
+    assert e.value.status == _lib.ERR_DEVICE
+    r = 0 if first else 2
+    rows = slice(int(b.off[r]), int(b.off[r + 1]))
+    assert (out[rows] == 0).all() and (lse[rows] == -math.inf).all()
+    whole, whole_lse = b.run()
+    serving.synchronize()
+    b.check(whole, whole_lse)
+    # the bad request's rows of the unbounded call, the others' of the bounded one
+    out[rows], lse[rows] = whole[rows], whole_lse[rows]
+    b.check(out, lse)
