@@ -93,7 +93,11 @@ int nb2_device_open(int ordinal, nb2_device** out);
  * device error word of its own: work of this context is ordered with the
  * caller's other work on that stream, and contexts of different streams share
  * no scratch. The stream must outlive the context. Any row takes it in place of
- * nb2_device_open's. One host thread at a time per context. */
+ * nb2_device_open's. One host thread at a time per context. The caller may
+ * capture the stream in a CUDA graph once the context is made: the graph then
+ * has a workspace of its own (up to 39 MB, taken back when the graph and its
+ * executable are gone) and may be replayed on any stream beside other work; two
+ * executables made of one graph share it and may not run at once. */
 int nb2_device_on_stream(int ordinal, void* stream, nb2_device** out);
 /* Waits for the stream, then frees a context from nb2_device_on_stream (null
  * is a no-op; a context from nb2_device_open is NB2_ERR_INVALID). */

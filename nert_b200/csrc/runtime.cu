@@ -5,7 +5,9 @@
 
 #include <cuda.h>
 
+#include <algorithm>
 #include <array>
+#include <atomic>
 #include <cstring>
 #include <memory>
 
@@ -88,6 +90,57 @@ void make_error_word(nb2_device* dev) {
     check_cuda(cudaStreamSynchronize(dev->stream), "cudaStreamSynchronize");
 }
 
+// Memory of graphs that callers capture: a block belongs to one graph, which
+// gives it back when it and its executables are gone, and is then the next
+// capture's. Blocks are never freed: the release runs on a thread of the
+// driver's, where no CUDA call may be made.
+struct GraphBlock {
+    void* ptr = nullptr;
+    size_t bytes = 0;
+    std::atomic<bool> used{false};
+};
+std::mutex g_graph_mu;
+std::array<std::vector<GraphBlock*>, 64>& graph_blocks() {
+    static auto* blocks = new std::array<std::vector<GraphBlock*>, 64>; // outlives every release
+    return *blocks;
+}
+
+void CUDART_CB release_graph_block(void* block) { static_cast<GraphBlock*>(block)->used = false; }
+
+// At least `bytes` on the current GPU for the life of `graph`, during its capture.
+void* graph_memory(int ordinal, cudaGraph_t graph, size_t bytes) {
+    std::lock_guard<std::mutex> lock(g_graph_mu);
+    auto& blocks = graph_blocks()[ordinal];
+    GraphBlock* block = nullptr;
+    for (GraphBlock* b : blocks) { // the smallest that is free and large enough
+        if (!b->used && b->bytes >= bytes && (block == nullptr || b->bytes < block->bytes)) {
+            block = b;
+        }
+    }
+    if (block == nullptr) {
+        auto fresh = std::make_unique<GraphBlock>();
+        // an allocation is no work of the stream: it may be made during a capture by a thread that says so
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        check_cuda(cudaThreadExchangeStreamCaptureMode(&mode), "cudaThreadExchangeStreamCaptureMode");
+        const cudaError_t e = cudaMalloc(&fresh->ptr, bytes);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        check_cuda(e, "cudaMalloc(graph workspace)");
+        fresh->bytes = bytes;
+        blocks.push_back(fresh.get());
+        block = fresh.release();
+    }
+    cudaUserObject_t owner = nullptr;
+    check_cuda(cudaUserObjectCreate(&owner, block, release_graph_block, 1, cudaUserObjectNoDestructorSync),
+               "cudaUserObjectCreate");
+    block->used = true;
+    const cudaError_t e = cudaGraphRetainUserObject(graph, owner, 1, cudaGraphUserObjectMove);
+    if (e != cudaSuccess) {
+        cudaUserObjectRelease(owner, 1);
+        check_cuda(e, "cudaGraphRetainUserObject");
+    }
+    return block->ptr;
+}
+
 } // namespace
 
 nb2_device* device(int ordinal) {
@@ -145,8 +198,36 @@ nb2_device::nb2_device() : wait_bound(nb2::kDefaultWaitBoundCycles) {}
 
 void nb2_device::make_current() const { nb2::check_cuda(cudaSetDevice(ordinal), "cudaSetDevice"); }
 
+cudaGraph_t nb2_device::callers_graph() {
+    if (!callers_stream) {
+        return nullptr;
+    }
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    cudaGraph_t graph = nullptr;
+    if (cudaStreamGetCaptureInfo(stream, &st, &id, &graph) != cudaSuccess) {
+        cudaGetLastError(); // the legacy stream while another stream captures
+        return nullptr;
+    }
+    if (st != cudaStreamCaptureStatusActive) {
+        return nullptr;
+    }
+    if (captured.id != id) {
+        captured = Captured{};
+        captured.id = id;
+    }
+    return graph;
+}
+
 void* nb2_device::scratch(size_t bytes) {
     bytes = (bytes + 255) & ~size_t(255);
+    if (const cudaGraph_t graph = callers_graph()) {
+        if (bytes > captured.workspace_bytes) {
+            captured.workspace = nb2::graph_memory(ordinal, graph, bytes);
+            captured.workspace_bytes = bytes;
+        }
+        return captured.workspace;
+    }
     if (bytes <= workspace_bytes) {
         return workspace;
     }
@@ -154,12 +235,6 @@ void* nb2_device::scratch(size_t bytes) {
         nb2::fail(nb2::kStatusInvalid, "workspace must be sized before CUDA-graph capture");
     }
     nb2::check_cuda(cudaStreamSynchronize(stream), "cudaStreamSynchronize(workspace grow)");
-    if (workspace != nullptr && callers_stream) {
-        // a graph that the caller captured may still hold its address
-        retired_split.push_back(workspace);
-        workspace = nullptr;
-        workspace_bytes = 0;
-    }
     if (workspace != nullptr) {
         nb2::check_cuda(cudaFree(workspace), "cudaFree(workspace)");
         workspace = nullptr;
@@ -175,6 +250,13 @@ void* nb2_device::split_scratch(size_t bytes) {
     bytes = (bytes + 255) & ~size_t(255);
     if (no_grow) {
         return nullptr; // a no-allocation call never depends on this shared buffer
+    }
+    if (const cudaGraph_t graph = callers_graph()) {
+        if (bytes > captured.split_ws_bytes) {
+            captured.split_ws = nb2::graph_memory(ordinal, graph, bytes);
+            captured.split_ws_bytes = bytes;
+        }
+        return captured.split_ws;
     }
     if (bytes <= split_ws_bytes) {
         return split_ws;
@@ -194,6 +276,17 @@ void* nb2_device::split_scratch(size_t bytes) {
 }
 
 uint32_t* nb2_device::tickets(size_t n) {
+    if (const cudaGraph_t graph = callers_graph()) {
+        if (n > captured.ticket_count) {
+            const size_t count = std::max<size_t>(n, 4096);
+            captured.ticket_ws = static_cast<uint32_t*>(nb2::graph_memory(ordinal, graph, count * sizeof(uint32_t)));
+            captured.ticket_count = count;
+            // a node of the graph: each replay begins with zeros
+            nb2::check_cuda(cudaMemsetAsync(captured.ticket_ws, 0, count * sizeof(uint32_t), stream),
+                            "cudaMemsetAsync(graph tickets)");
+        }
+        return captured.ticket_ws;
+    }
     if (n <= ticket_count) {
         return ticket_ws;
     }

@@ -90,6 +90,19 @@ struct nb2_device {
     uint32_t* ticket_ws = nullptr;
     size_t ticket_count = 0;
     std::vector<void*> retired_tickets;
+    // What the caller's CUDA-graph capture of this context's stream uses in
+    // place of the buffers above: its graph may be replayed on any stream,
+    // beside other work of this context. The memory is the graph's, for its
+    // life.
+    struct Captured {
+        unsigned long long id = 0;
+        void* workspace = nullptr;
+        size_t workspace_bytes = 0;
+        void* split_ws = nullptr;
+        size_t split_ws_bytes = 0;
+        uint32_t* ticket_ws = nullptr;
+        size_t ticket_count = 0;
+    } captured;
     // clock64 ticks after which a tensor-core kernel's mbarrier wait gives
     // up, records a device error and unwinds (default about one second)
     long long wait_bound;
@@ -111,7 +124,8 @@ struct nb2_device {
     void make_current() const;
     // Returns a workspace of at least `bytes` (256-B aligned). Growing it
     // synchronises the stream first, so pointers from earlier calls stay
-    // valid until the kernels that use them have finished.
+    // valid until the kernels that use them have finished. In a capture of
+    // the caller's it is that capture's own, as the two below.
     void* scratch(size_t bytes);
     // Buffer for split-K partial sums of at least `bytes`, or nullptr inside a
     // call that must not allocate, or when it would have to grow inside a
@@ -123,6 +137,9 @@ struct nb2_device {
     // Whether the stream is inside a CUDA-graph capture (the engine's or a
     // caller's own), where nothing may be allocated or waited for.
     bool in_capture() const;
+    // The graph that the caller captures on this context's stream, null where
+    // none is; `captured` is then that capture's.
+    cudaGraph_t callers_graph();
     // Reads and clears the device error word (synchronises the stream).
     int take_device_error();
 };

@@ -7,7 +7,9 @@ the stream; every computation is a kernel of libnert_b200.so.
 Unlike the wrappers of ``nert_b200.ops``, these launch on torch's current
 stream (through one context a stream, made on first use) and return without
 synchronising, so a step can be queued, overlapped or captured in a CUDA graph
-(after one uncaptured call on that stream, which sizes the workspace).
+(after one uncaptured call, or ``context()``, on the capturing stream). A captured
+graph has a workspace of its own, so it may be replayed on any stream, beside
+other graphs and calls; one replay at a time of each, as CUDA has it.
 Arguments that the host can see are checked before the launch (``ValueError``,
 or ``NB2Error`` from the library); values on the device (lengths, blocks, slots,
 token ids) are checked by the kernels, and ``synchronize()`` raises what they

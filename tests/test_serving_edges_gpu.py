@@ -14,7 +14,7 @@ import torch
 
 from conftest import ROOT
 from nert_b200 import _lib, serving
-from test_serving_gpu import Batch
+from test_serving_gpu import Batch, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +100,65 @@ def test_tree_attention_request_past_its_bound_beside_good_ones(cuda, dtype, dim
     # the bad request's rows of the unbounded call, the others' of the bounded one
     out[rows], lse[rows] = whole[rows], whole_lse[rows]
     b.check(out, lse)
+
+
+def _in_graph(stream, call, n=1):
+    """A graph of n calls captured on a stream that has a context, and its last outputs."""
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        serving.context()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=stream):
+            for _ in range(n):
+                out = call()
+    return g, out
+
+
+@pytest.mark.parametrize("dtype,olds,news", [
+    ("bf16", [900, 2000, 60], [1, 1, 1]), ("f32", [700, 4000], [9, 12]), ("bf16", [3000, 900, 5000], [40, 33, 64]),
+])
+def test_graphs_of_one_stream_replayed_at_once(cuda, dtype, olds, news):
+    """Graphs captured on one stream, replayed on two others beside calls on the first: each has pieces and
+    tickets of its own. Every batch has items that several CTAs share."""
+    bs = [Batch(olds, news, 16, 4, 128, 16, dtype, seed=s) for s in range(3)]
+    args = [(b.q, b.kc, b.vc, i32(b.table), i32(b.total), i32(b.off)) for b in bs]
+    calls = [lambda a=a, b=b: serving.tree_attention(*a, tree_mask=b.mask, max_new=max(news), return_lse=True) for a, b in zip(args, bs)]
+    want = [c() for c in calls]
+    serving.synchronize()
+    for (out, lse), b in zip(want, bs):
+        b.check(out, lse)
+    first, others = torch.cuda.Stream(), [torch.cuda.Stream() for _ in range(2)]
+    graphs = [_in_graph(first, c, 20) for c in calls[:2]]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for (g, _), s in zip(graphs, others):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(first):
+            for _ in range(20):
+                eager = calls[2]()
+        torch.cuda.synchronize()
+        for (out, lse), (o, l) in zip([graphs[0][1], graphs[1][1], eager], want):
+            assert torch.equal(out, o) and torch.equal(lse, l)
+            out.zero_(), lse.zero_()
+    with torch.cuda.stream(first):
+        serving.synchronize()
+
+
+def test_graphs_give_their_workspace_back(cuda):
+    """A workspace belongs to a graph as long as it lives: the next capture takes one that a dead graph had."""
+    b = Batch([30000], [12], 4, 1, 128, 16, "bf16")
+    args = (b.q, b.kc, b.vc, i32(b.table), i32(b.total), i32(b.off))
+    want = serving.tree_attention(*args, tree_mask=b.mask, max_new=12)
+    stream = torch.cuda.Stream()
+    left = []
+    for _ in range(40):
+        g, out = _in_graph(stream, lambda: serving.tree_attention(*args, tree_mask=b.mask, max_new=12))
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        del g, out
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        left.append(torch.cuda.mem_get_info()[0])
+    assert left[5] - left[-1] < 32 << 20  # one workspace is 10 MB
