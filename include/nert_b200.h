@@ -97,7 +97,9 @@ int nb2_device_open(int ordinal, nb2_device** out);
  * capture the stream in a CUDA graph once the context is made: the graph then
  * has a workspace of its own (up to 39 MB, taken back when the graph and its
  * executable are gone) and may be replayed on any stream beside other work; two
- * executables made of one graph share it and may not run at once. */
+ * executables made of one graph share it and may not run at once. Device errors
+ * of replayed graphs are kept by GPU: the next synchronisation of any context of
+ * this kind reports them. */
 int nb2_device_on_stream(int ordinal, void* stream, nb2_device** out);
 /* Waits for the stream, then frees a context from nb2_device_on_stream (null
  * is a no-op; a context from nb2_device_open is NB2_ERR_INVALID). */

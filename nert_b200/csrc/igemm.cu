@@ -1360,7 +1360,7 @@ void launch(nb2_device* dev, Args& a, int64_t n_per_z, int64_t z, const float* p
     CUtensorMap hi, lo;
     make_tmap(&hi, packed, kpad, rows_total, bn);
     make_tmap(&lo, packed + rows_total * kpad, kpad, rows_total, bn);
-    a.err = dev->err_word;
+    a.err = dev->error_word();
     a.wait_bound = dev->wait_bound;
     a.zcount = static_cast<int>(z);
     auto al16 = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };

@@ -436,7 +436,7 @@ void attention(nb2_device* dev, const AttnGeom& g, const float* q, const float* 
         }
         attr_bytes[dev->ordinal] = smem;
     }
-    AttnArgs a{g, q, k, v, out, dev->err_word, dev->wait_bound};
+    AttnArgs a{g, q, k, v, out, dev->error_word(), dev->wait_bound};
     // a division by a power of two is the multiplication by its exact
     // reciprocal (both are the correctly rounded s / c)
     if (a.g.scale_mode == 2) {

@@ -316,11 +316,11 @@ void binary(nb2_device* dev, int op, int dtype, const void* a, const std::vector
     if (dtype == kF32) {
         binary_bcast_kernel<float><<<grid_for(dev, n), 256, 0, dev->stream>>>(
             op, static_cast<const float*>(a), static_cast<const float*>(b), static_cast<float*>(y), n, s,
-            dev->err_word);
+            dev->error_word());
     } else if (dtype == kI64) {
         binary_bcast_kernel<long long><<<grid_for(dev, n), 256, 0, dev->stream>>>(
             op, static_cast<const long long*>(a), static_cast<const long long*>(b), static_cast<long long*>(y), n, s,
-            dev->err_word);
+            dev->error_word());
     } else {
         fail(kStatusUnsupported, "binary: unsupported dtype");
     }

@@ -664,15 +664,15 @@ void gather(nb2_device* dev, const void* x, const int64_t* idx, void* y, int64_t
     const unsigned g = blocks_for(dev, total);
     if (elem_bytes == 4) {
         gather_kernel<float><<<g, 256, 0, dev->stream>>>(static_cast<const float*>(x), idx, static_cast<float*>(y),
-                                                         outer, axis_len, inner, n_idx, dev->err_word);
+                                                         outer, axis_len, inner, n_idx, dev->error_word());
     } else if (elem_bytes == 8) {
         gather_kernel<long long><<<g, 256, 0, dev->stream>>>(static_cast<const long long*>(x), idx,
                                                              static_cast<long long*>(y), outer, axis_len, inner,
-                                                             n_idx, dev->err_word);
+                                                             n_idx, dev->error_word());
     } else {
         gather_kernel<uint8_t><<<g, 256, 0, dev->stream>>>(static_cast<const uint8_t*>(x), idx,
                                                            static_cast<uint8_t*>(y), outer, axis_len, inner, n_idx,
-                                                           dev->err_word);
+                                                           dev->error_word());
     }
     check_cuda(cudaGetLastError(), "gather launch");
 }

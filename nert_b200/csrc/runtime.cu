@@ -90,6 +90,29 @@ void make_error_word(nb2_device* dev) {
     check_cuda(cudaStreamSynchronize(dev->stream), "cudaStreamSynchronize");
 }
 
+// Error words of the graphs that callers captured, one a GPU, made with its
+// first context on a caller's stream.
+struct GraphErrors {
+    int* word = nullptr;
+    std::atomic<bool> used{false}; // a graph holds it
+};
+std::array<GraphErrors, 64> g_graph_errors;
+
+void make_graph_error_word(nb2_device* dev) {
+    std::lock_guard<std::mutex> lock(g_devices_mu);
+    GraphErrors& e = g_graph_errors[dev->ordinal];
+    if (e.word == nullptr) {
+        int* word = nullptr;
+        check_cuda(cudaMalloc(&word, 256), "cudaMalloc(graph error word)");
+        check_cuda(cudaMemsetAsync(word, 0, 256, dev->stream), "cudaMemsetAsync(graph error word)");
+        check_cuda(cudaStreamSynchronize(dev->stream), "cudaStreamSynchronize");
+        e.word = word;
+    }
+}
+
+// Takes a word that other streams may be writing.
+__global__ void take_word_kernel(int* word, int* to) { *to = atomicExch(word, 0); }
+
 // Memory of graphs that callers capture: a block belongs to one graph, which
 // gives it back when it and its executables are gone, and is then the next
 // capture's. Blocks are never freed: the release runs on a thread of the
@@ -168,6 +191,7 @@ nb2_device* device_on_stream(int ordinal, cudaStream_t stream) {
         fail(kStatusInvalid, "a context must be made before its stream's CUDA-graph capture");
     }
     make_error_word(dev.get());
+    make_graph_error_word(dev.get());
     return dev.release();
 }
 
@@ -317,14 +341,29 @@ bool nb2_device::in_capture() const {
     return st != cudaStreamCaptureStatusNone;
 }
 
+int* nb2_device::error_word() {
+    if (callers_graph() == nullptr) {
+        return err_word;
+    }
+    nb2::GraphErrors& e = nb2::g_graph_errors[ordinal];
+    e.used = true;
+    return e.word;
+}
+
 int nb2_device::take_device_error() {
-    int code = 0;
-    nb2::check_cuda(cudaMemcpyAsync(&code, err_word, sizeof(int), cudaMemcpyDeviceToHost, stream),
+    int codes[2] = {0, 0}; // this context's, replayed graphs'
+    const nb2::GraphErrors& graphs = nb2::g_graph_errors[ordinal];
+    const bool with_graphs = callers_stream && graphs.used;
+    if (with_graphs) {
+        nb2::take_word_kernel<<<1, 1, 0, stream>>>(graphs.word, err_word + 1);
+        nb2::check_cuda(cudaGetLastError(), "error word launch");
+    }
+    nb2::check_cuda(cudaMemcpyAsync(codes, err_word, (with_graphs ? 2 : 1) * sizeof(int), cudaMemcpyDeviceToHost, stream),
                     "cudaMemcpyAsync(error word)");
     nb2::check_cuda(cudaStreamSynchronize(stream), "cudaStreamSynchronize");
-    if (code != 0) {
+    if (codes[0] != 0) {
         nb2::check_cuda(cudaMemsetAsync(err_word, 0, sizeof(int), stream), "cudaMemsetAsync(error word)");
         nb2::check_cuda(cudaStreamSynchronize(stream), "cudaStreamSynchronize");
     }
-    return code;
+    return codes[0] != 0 ? codes[0] : codes[1];
 }

@@ -140,7 +140,12 @@ struct nb2_device {
     // The graph that the caller captures on this context's stream, null where
     // none is; `captured` is then that capture's.
     cudaGraph_t callers_graph();
-    // Reads and clears the device error word (synchronises the stream).
+    // Where a launch records device errors: the context's word, or in a capture
+    // of the caller's the word of the GPU's replayed graphs, which every context
+    // on a caller's stream reads (the graph may be replayed on any of them).
+    int* error_word();
+    // Reads and clears the device error word, on a caller's stream also that of
+    // replayed graphs (synchronises the stream).
     int take_device_error();
 };
 

@@ -676,7 +676,7 @@ void tree_attention(nb2_device* dev, TreeAttnArgs a) {
     if (a.g.tokens == 0) {
         return;
     }
-    a.err = dev->err_word;
+    a.err = dev->error_word();
     if (tree_attention_tc_takes(a, dev->num_sms)) {
         tree_attention_tc(dev, a);
     } else if (a.g.dtype == kF32) {

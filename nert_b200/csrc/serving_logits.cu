@@ -348,7 +348,7 @@ void logits_process(nb2_device* dev, LogitsArgs a) {
     if (a.g.rows == 0) {
         return;
     }
-    a.err = dev->err_word;
+    a.err = dev->error_word();
     if (a.g.in_dtype == kF32) {
         pick_logits<float>(dev, a);
     } else if (a.g.in_dtype == kF16) {

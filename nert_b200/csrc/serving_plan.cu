@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PagePlanArgs a,
 } // namespace
 
 void page_plan(nb2_device* dev, PagePlanArgs a) {
-    a.err = dev->err_word;
+    a.err = dev->error_word();
     const int64_t parts = std::max<int64_t>(1, (a.g.tokens + kPlanTokens - 1) / kPlanTokens);
     const int64_t trees = a.parents != nullptr ? a.g.batch : 0;
     if (parts + trees > 0x7fffffffLL) {

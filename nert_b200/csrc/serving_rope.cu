@@ -263,7 +263,7 @@ void rope_append(nb2_device* dev, RopeArgs a) {
     if (a.g.tokens == 0) {
         return;
     }
-    a.err = dev->err_word;
+    a.err = dev->error_word();
     if (a.g.dtype == kF32) {
         pick_rope<float>(dev, a);
     } else if (a.g.dtype == kF16) {

@@ -47,7 +47,8 @@ _native = _load()
 
 def synchronize(device: torch.device | str = "cuda") -> None:
     """Waits for torch's current stream; raises what the kernels of this module
-    recorded on it (NB2Error with status ERR_DEVICE)."""
+    recorded on it, and what the GPU's replayed graphs did, on whatever stream
+    (NB2Error with status ERR_DEVICE)."""
     _native.synchronize(torch.device(device))
 
 

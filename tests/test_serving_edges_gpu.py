@@ -162,3 +162,35 @@ def test_graphs_give_their_workspace_back(cuda):
         torch.cuda.empty_cache()
         left.append(torch.cuda.mem_get_info()[0])
     assert left[5] - left[-1] < 32 << 20  # one workspace is 10 MB
+
+
+def test_errors_of_a_graph_replayed_on_another_stream(cuda):
+    """What a replayed graph records is raised where its stream is waited for, once, and not by the next replay."""
+    old, new, table = i32([3, 4]), i32([1, 1]), i32([[0], [1]])
+    free, stream = i32([2]), torch.cuda.Stream()
+    g, plan = _in_graph(stream, lambda: serving.page_plan(old, new, table, free, 16, 2))
+    g.replay()
+    serving.synchronize()
+    assert plan.slots.tolist() == [3, 20]
+    old.fill_(-1)
+    g.replay()
+    with pytest.raises(_lib.NB2Error) as e:
+        serving.synchronize()
+    assert e.value.status == _lib.ERR_DEVICE
+    serving.synchronize()
+    old.copy_(i32([5, 6]))
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(other):
+        g.replay()
+        serving.synchronize()
+    with torch.cuda.stream(stream):
+        serving.synchronize()
+    assert plan.slots.tolist() == [5, 22]
+    # a call's own error is its stream's, as before
+    with torch.cuda.stream(other):
+        serving.page_plan(i32([-1]), i32([1]), i32([[0]]), free, 16, 1)
+        torch.cuda.synchronize()
+    serving.synchronize()
+    with torch.cuda.stream(other), pytest.raises(_lib.NB2Error):
+        serving.synchronize()
