@@ -93,7 +93,8 @@ int nb2_device_open(int ordinal, nb2_device** out);
  * device error word of its own: work of this context is ordered with the
  * caller's other work on that stream, and contexts of different streams share
  * no scratch. The stream must outlive the context. Any row takes it in place of
- * nb2_device_open's. One host thread at a time per context. The caller may
+ * nb2_device_open's. One host thread at a time per context. A call makes the
+ * context's GPU current for its thread. The caller may
  * capture the stream in a CUDA graph once the context is made: the graph then
  * has a workspace of its own (up to 39 MB, taken back when the graph and its
  * executable are gone) and may be replayed on any stream beside other work; two

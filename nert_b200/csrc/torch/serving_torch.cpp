@@ -8,6 +8,7 @@
 
 #include "../../../include/nert_b200.h"
 
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
@@ -38,10 +39,19 @@ void check(int status) {
 
 #define NEED(cond, ...) TORCH_CHECK_VALUE(cond, __VA_ARGS__)
 
+// The GPU of a call, with its index.
+c10::Device gpu(c10::Device device) {
+    NEED(device.is_cuda(), "expected tensors on a GPU");
+    return device.has_index() ? device : c10::Device(c10::kCUDA, c10::cuda::current_device());
+}
+
+// The library makes a context's GPU current for the thread. Every function that
+// Python calls holds one of these, so that torch's current GPU is the caller's again after it.
+using OnGpu = c10::cuda::CUDAGuard;
+
 // The context of torch's current stream on the tensor's GPU, made on first use
 // and kept: torch hands out streams from fixed pools.
 nb2_device* context(c10::Device device) {
-    NEED(device.is_cuda(), "expected tensors on a GPU");
     const c10::cuda::CUDAStream s = c10::cuda::getCurrentCUDAStream(device.index());
     struct Entry {
         int device;
@@ -127,8 +137,9 @@ void* address(const OptTensor& t) { return t.has_value() ? t->data_ptr() : nullp
 std::tuple<Tensor, Tensor, Tensor, Tensor, OptTensor, Tensor>
 page_plan(const Tensor& seq_lens, const Tensor& new_lens, const Tensor& table, const Tensor& free_blocks,
           int64_t block_size, int64_t tokens, const OptTensor& parents, int64_t mask_words, const OptTensor& free_head) {
-    nb2_device* dev = context(seq_lens.device());
-    const c10::Device on = seq_lens.device();
+    const c10::Device on = gpu(seq_lens.device());
+    const OnGpu guard(on);
+    nb2_device* dev = context(on);
     const int32_t* old = ints(seq_lens, "seq_lens", on);
     const int32_t* fresh = ints(new_lens, "new_lens", on);
     const int32_t* pool = ints(free_blocks, "free_blocks", on);
@@ -175,8 +186,9 @@ std::tuple<Tensor, OptTensor> rope_append(const Tensor& q, const Tensor& k, cons
                                           const Tensor& positions, const std::optional<py::bytes>& axis_of, int axes,
                                           bool interleaved, const OptTensor& slots, const OptTensor& k_cache,
                                           const OptTensor& v_cache, const OptTensor& q_out, const OptTensor& k_out) {
-    nb2_device* dev = context(q.device());
-    const c10::Device on = q.device();
+    const c10::Device on = gpu(q.device());
+    const OnGpu guard(on);
+    nb2_device* dev = context(on);
     NEED(q.dim() == 3, "q: expected [tokens, heads, head_dim]");
     nb2_rope_geom g{};
     g.dtype = dtype_code(q, "q");
@@ -260,8 +272,9 @@ std::tuple<Tensor, OptTensor> tree_attention(const Tensor& q, const Tensor& k_ca
                                              const Tensor& table, const Tensor& seq_lens, const Tensor& token_offsets,
                                              const OptTensor& tree_mask, std::optional<int64_t> max_new,
                                              std::optional<double> scale, bool return_lse, const OptTensor& out) {
-    nb2_device* dev = context(q.device());
-    const c10::Device on = q.device();
+    const c10::Device on = gpu(q.device());
+    const OnGpu guard(on);
+    nb2_device* dev = context(on);
     NEED(q.dim() == 3, "q: expected [tokens, heads, head_dim]");
     nb2_tree_attn_geom g{};
     g.dtype = dtype_code(q, "q");
@@ -328,8 +341,9 @@ Tensor logits_process(const Tensor& logits, const List& prompt, const List& outp
                       const std::optional<std::tuple<Tensor, Tensor, Tensor>>& bias,
                       const std::optional<std::tuple<Tensor, OptTensor>>& grammar, std::optional<at::ScalarType> out_dtype,
                       const OptTensor& out, std::optional<int64_t> n_requests) {
-    nb2_device* dev = context(logits.device());
-    const c10::Device on = logits.device();
+    const c10::Device on = gpu(logits.device());
+    const OnGpu guard(on);
+    nb2_device* dev = context(on);
     NEED(logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1), "logits: expected [rows, vocab]");
     nb2_logits_geom g{};
     g.rows = logits.size(0);
@@ -396,9 +410,17 @@ Tensor logits_process(const Tensor& logits, const List& prompt, const List& outp
     return o;
 }
 
-void synchronize(c10::Device device) { check(nb2_device_synchronize(context(device))); }
+void synchronize(c10::Device device) {
+    const c10::Device on = gpu(device);
+    const OnGpu guard(on);
+    check(nb2_device_synchronize(context(on)));
+}
 
-int64_t context_address(c10::Device device) { return reinterpret_cast<int64_t>(context(device)); }
+int64_t context_address(c10::Device device) {
+    const c10::Device on = gpu(device);
+    const OnGpu guard(on);
+    return reinterpret_cast<int64_t>(context(on));
+}
 
 } // namespace
 

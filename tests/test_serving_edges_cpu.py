@@ -29,3 +29,14 @@ def test_tensor_memory_loads_wait_in_their_own_statement():
                     seen += 1
                     assert "tcgen05.wait::ld" in statement, f"{os.path.basename(path)}: {statement}"
     assert seen >= 4
+
+
+def test_the_python_module_guards_the_current_gpu():
+    """Each function that Python calls restores the current GPU (with one GPU no run can show it)."""
+    with open(os.path.join(ROOT, "nert_b200", "csrc", "torch", "serving_torch.cpp")) as f:
+        source = f.read()
+    functions = re.findall(r'm\.def\("\w+", &(\w+)\)', source)
+    assert len(functions) == 6
+    for name in functions:
+        body = re.search(r"^[\w:<>, \n]*\b%s\([^{;]*\{\n(.*?)^\}" % name, source, re.S | re.M).group(1)
+        assert "OnGpu guard(" in body and ("context(" not in body or body.index("OnGpu guard(") < body.index("context(")), name

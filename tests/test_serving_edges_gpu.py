@@ -194,3 +194,23 @@ def test_errors_of_a_graph_replayed_on_another_stream(cuda):
     serving.synchronize()
     with torch.cuda.stream(other), pytest.raises(_lib.NB2Error):
         serving.synchronize()
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="two GPUs: the current one and another")
+def test_the_current_gpu_stays_the_callers(cuda):
+    """Calls on another GPU's tensors leave torch's current GPU as it was, with the first use of a stream or later."""
+    there = torch.device("cuda:1")
+    ints = lambda x: torch.tensor(x, device=there, dtype=torch.int32)  # noqa: E731
+    half = lambda *shape: torch.zeros(*shape, device=there, dtype=torch.float16)  # noqa: E731
+    torch.cuda.set_device(0)
+    for _ in range(2):
+        for call in (
+            lambda: serving.context(there),
+            lambda: serving.page_plan(ints([0]), ints([1]), ints([[0]]), ints([0]), 16, 1),
+            lambda: serving.rope_append(half(1, 1, 8), half(1, 1, 8), None, torch.zeros(4, 8, device=there), ints([0])),
+            lambda: serving.tree_attention(half(1, 1, 64), half(1, 16, 1, 64), half(1, 16, 1, 64), ints([[0]]), ints([1]), ints([0, 1])),
+            lambda: serving.logits_process(half(1, 8)),
+            lambda: serving.synchronize(there),
+        ):
+            call()
+            assert torch.cuda.current_device() == 0 and torch.zeros(1, device="cuda").device.index == 0
