@@ -351,6 +351,8 @@ int* nb2_device::error_word() {
 }
 
 int nb2_device::take_device_error() {
+    // two threads that wait for one context take turns: each reads the words, then clears them
+    std::lock_guard<std::mutex> lock(mu);
     int codes[2] = {0, 0}; // this context's, replayed graphs'
     const nb2::GraphErrors& graphs = nb2::g_graph_errors[ordinal];
     const bool with_graphs = callers_stream && graphs.used;

@@ -413,7 +413,13 @@ Tensor logits_process(const Tensor& logits, const List& prompt, const List& outp
 void synchronize(c10::Device device) {
     const c10::Device on = gpu(device);
     const OnGpu guard(on);
-    check(nb2_device_synchronize(context(on)));
+    nb2_device* dev = context(on);
+    int status;
+    {
+        py::gil_scoped_release free; // other threads run while this one waits
+        status = nb2_device_synchronize(dev);
+    }
+    check(status);
 }
 
 int64_t context_address(c10::Device device) {

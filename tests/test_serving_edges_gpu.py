@@ -7,6 +7,8 @@ import math
 import os
 import subprocess
 import sys
+import threading
+import time
 
 import numpy as np
 import pytest
@@ -214,3 +216,40 @@ def test_the_current_gpu_stays_the_callers(cuda):
         ):
             call()
             assert torch.cuda.current_device() == 0 and torch.zeros(1, device="cuda").device.index == 0
+
+
+def test_other_threads_run_while_one_waits(cuda):
+    """synchronize() waits without the interpreter's lock, in several threads too, and each error is raised once."""
+    serving.synchronize()
+    turns, stop = [0], threading.Event()
+
+    def count():
+        while not stop.wait(0.001):
+            turns[0] += 1
+
+    other = threading.Thread(target=count)
+    other.start()
+    try:
+        torch.cuda._sleep(600_000_000)  # about 0.3 s
+        before = turns[0]
+        serving.synchronize()
+        assert turns[0] - before > 20
+    finally:
+        stop.set()
+        other.join()
+
+    raised = []
+
+    def wait():
+        try:
+            serving.synchronize()
+        except _lib.NB2Error as e:
+            raised.append(e.status)
+
+    for _ in range(5):
+        serving.page_plan(i32([-1]), i32([1]), i32([[0]]), i32([0]), 16, 1)
+        threads = [threading.Thread(target=wait) for _ in range(4)]
+        [t.start() for t in threads]
+        [t.join() for t in threads]
+        assert raised == [_lib.ERR_DEVICE]
+        raised.clear()
