@@ -46,6 +46,14 @@ constexpr int64_t kMaxI32 = 0x7fffffff;
 
 bool in_i32(int64_t v) { return v >= 0 && v <= kMaxI32; }
 
+// The stride of a dimension of one element says nothing, whatever it is: a caller's views may hold any. It becomes a
+// head's length, which every check of alignment allows.
+void level(int64_t extent, int64_t& stride, int64_t head_dim) {
+    if (extent <= 1) {
+        stride = head_dim;
+    }
+}
+
 } // namespace
 
 extern "C" {
@@ -113,8 +121,24 @@ int nb2_rope_append(nb2_device* dev, const nb2_rope_geom* g, const void* q, cons
         need(k_cache != nullptr || k_out != nullptr, "RopeAppend: the keys have nowhere to go");
         need(k_cache == nullptr || (g->block_size > 0 && g->block_size <= kMaxI32 && in_i32(g->num_blocks)),
              "RopeAppend: bad cache extents");
+        nb2_rope_geom e = *g;
+        for (int64_t* s : {&e.q_stride, &e.k_stride, &e.v_stride, &e.qo_stride, &e.ko_stride}) {
+            level(g->tokens, *s, g->head_dim);
+        }
+        for (int64_t* s : {&e.q_head_stride, &e.qo_head_stride}) {
+            level(g->q_heads, *s, g->head_dim);
+        }
+        for (int64_t* s : {&e.k_head_stride, &e.v_head_stride, &e.ko_head_stride, &e.kc_head_stride, &e.vc_head_stride}) {
+            level(g->kv_heads, *s, g->head_dim);
+        }
+        for (int64_t* s : {&e.kc_block_stride, &e.vc_block_stride}) {
+            level(g->num_blocks, *s, g->head_dim);
+        }
+        for (int64_t* s : {&e.kc_place_stride, &e.vc_place_stride}) {
+            level(g->block_size, *s, g->head_dim);
+        }
         bind(dev);
-        rope_append(dev, RopeArgs{*g, q, k, v, table, positions, slots, q_out, k_out, k_cache, v_cache, nullptr});
+        rope_append(dev, RopeArgs{e, q, k, v, table, positions, slots, q_out, k_out, k_cache, v_cache, nullptr});
     });
 }
 
@@ -149,17 +173,32 @@ int nb2_tree_attention(nb2_device* dev, const nb2_tree_attn_geom* g, const void*
         need(g->batch == 0 || total_lens != nullptr, "TreeAttention: null buffer");
         need(g->batch == 0 || g->table_blocks == 0 || block_table != nullptr, "TreeAttention: null buffer");
         need(g->num_blocks == 0 || (k_cache && v_cache), "TreeAttention: null buffer");
+        nb2_tree_attn_geom e = *g;
+        for (int64_t* s : {&e.q_stride, &e.o_stride}) {
+            level(g->tokens, *s, g->head_dim);
+        }
+        for (int64_t* s : {&e.q_head_stride, &e.o_head_stride}) {
+            level(g->q_heads, *s, g->head_dim);
+        }
+        for (int64_t* s : {&e.kc_head_stride, &e.vc_head_stride}) {
+            level(g->kv_heads, *s, g->head_dim);
+        }
+        for (int64_t* s : {&e.kc_block_stride, &e.vc_block_stride}) {
+            level(g->num_blocks, *s, g->head_dim);
+        }
+        for (int64_t* s : {&e.kc_place_stride, &e.vc_place_stride}) {
+            level(g->block_size, *s, g->head_dim);
+        }
         const int64_t unit = 16 / dtype_bytes(g->dtype);
-        for (int64_t s : {g->q_stride, g->q_head_stride, g->o_stride, g->o_head_stride, g->kc_block_stride,
-                          g->kc_place_stride, g->kc_head_stride, g->vc_block_stride, g->vc_place_stride,
-                          g->vc_head_stride}) {
+        for (int64_t s : {e.q_stride, e.q_head_stride, e.o_stride, e.o_head_stride, e.kc_block_stride, e.kc_place_stride,
+                          e.kc_head_stride, e.vc_block_stride, e.vc_place_stride, e.vc_head_stride}) {
             need(s % unit == 0, "TreeAttention: strides must be multiples of 16 bytes");
         }
         for (const void* p : {q, k_cache, v_cache, static_cast<const void*>(out)}) {
             need((reinterpret_cast<uintptr_t>(p) & 15) == 0, "TreeAttention: buffers must be 16-byte aligned");
         }
         bind(dev);
-        tree_attention(dev, TreeAttnArgs{*g, q, k_cache, v_cache, block_table, total_lens, token_offsets,
+        tree_attention(dev, TreeAttnArgs{e, q, k_cache, v_cache, block_table, total_lens, token_offsets,
                                          reinterpret_cast<const uint32_t*>(tree_mask), out, lse, nullptr});
     });
 }

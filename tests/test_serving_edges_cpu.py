@@ -9,7 +9,7 @@ import re
 import pytest
 
 from conftest import ROOT
-from test_serving_cpu import ROPE, call, rope
+from test_serving_cpu import ATTN, ROPE, attn, call, rope
 
 
 @pytest.mark.parametrize("geom", [rope(block_size=2**31), rope(block_size=2**32), rope(num_blocks=2**31), rope(num_blocks=-1)])
@@ -40,3 +40,17 @@ def test_the_python_module_guards_the_current_gpu():
     for name in functions:
         body = re.search(r"^[\w:<>, \n]*\b%s\([^{;]*\{\n(.*?)^\}" % name, source, re.S | re.M).group(1)
         assert "OnGpu guard(" in body and ("context(" not in body or body.index("OnGpu guard(") < body.index("context(")), name
+
+
+ONES = [dict(tokens=1, q_stride=257, o_stride=3), dict(q_heads=1, kv_heads=1, q_head_stride=1, o_head_stride=7),
+        dict(kv_heads=1, kc_head_stride=1, vc_head_stride=0), dict(num_blocks=1, kc_block_stride=5, vc_block_stride=1),
+        dict(block_size=1, kc_place_stride=3, vc_place_stride=1)]
+
+
+@pytest.mark.parametrize("one", ONES)
+def test_tree_attention_takes_any_stride_of_a_dimension_of_one(one):
+    """Past its checks the call asks for its device."""
+    assert call("nb2_tree_attention", attn(**one), *ATTN) == (-1, "null device")
+    two = {n: 2 for n in ("tokens", "q_heads", "kv_heads", "num_blocks", "block_size") if n in one}
+    got, msg = call("nb2_tree_attention", attn(**(one | two)), *ATTN)
+    assert got == -1 and "16 bytes" in msg

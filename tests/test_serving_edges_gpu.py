@@ -253,3 +253,35 @@ def test_other_threads_run_while_one_waits(cuda):
         [t.join() for t in threads]
         assert raised == [_lib.ERR_DEVICE]
         raised.clear()
+
+
+def _odd_ones(x, *dims):
+    """x with a stride of 3 in those of its dimensions that have one element."""
+    return x.as_strided(x.shape, [3 if d in dims and n == 1 else s for d, (s, n) in enumerate(zip(x.stride(), x.shape))])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("olds,news,hq,hkv,block", [
+    ([20], [1], 1, 1, 1), ([70, 5], [2, 9], 4, 1, 16), ([3], [9], 8, 1, 16), ([300], [90], 1, 1, 16), ([10], [100], 2, 1, 256),
+])
+def test_any_stride_of_a_dimension_of_one(cuda, dtype, olds, news, hq, hkv, block):
+    b = Batch(olds, news, hq, hkv, 64, block, dtype)
+    want, want_lse = b.run()
+    serving.synchronize()
+    b.check(want, want_lse)
+    if block == 256:  # one block holds the request
+        b.kc, b.vc = (c[int(b.table[0, 0]):][:1] for c in (b.kc, b.vc))
+        b.table[:] = 0
+    b.q = _odd_ones(b.q, 0, 1)
+    b.kc, b.vc = _odd_ones(b.kc, 0, 1, 2), _odd_ones(b.vc, 0, 1, 2)
+    out, lse = b.run(out=_odd_ones(torch.empty_like(want), 0, 1))
+    serving.synchronize()
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+    # and the rotary row's, in values equal to those of plain views
+    n, pos, table = b.q.shape[0], i32(np.arange(b.q.shape[0])), torch.randn(b.q.shape[0], 64, device="cuda")
+    k = torch.randn(n, 1, 64, device="cuda").to(b.q.dtype)
+    q0, k0 = serving.rope_append(b.q.contiguous(), k, None, table, pos)
+    q1, k1 = serving.rope_append(b.q, _odd_ones(k, 0, 1), None, table, pos)
+    serving.synchronize()
+    assert torch.equal(q0, q1) and torch.equal(k0, k1)
