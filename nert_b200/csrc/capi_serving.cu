@@ -137,6 +137,10 @@ int nb2_rope_append(nb2_device* dev, const nb2_rope_geom* g, const void* q, cons
         for (int64_t* s : {&e.kc_place_stride, &e.vc_place_stride}) {
             level(g->block_size, *s, g->head_dim);
         }
+        need(q_out != q || (e.qo_stride == e.q_stride && e.qo_head_stride == e.q_head_stride),
+             "RopeAppend: in place needs equal strides");
+        need(k_out != k || (e.ko_stride == e.k_stride && e.ko_head_stride == e.k_head_stride),
+             "RopeAppend: in place needs equal strides");
         bind(dev);
         rope_append(dev, RopeArgs{e, q, k, v, table, positions, slots, q_out, k_out, k_cache, v_cache, nullptr});
     });

@@ -54,3 +54,17 @@ def test_tree_attention_takes_any_stride_of_a_dimension_of_one(one):
     two = {n: 2 for n in ("tokens", "q_heads", "kv_heads", "num_blocks", "block_size") if n in one}
     got, msg = call("nb2_tree_attention", attn(**(one | two)), *ATTN)
     assert got == -1 and "16 bytes" in msg
+
+
+@pytest.mark.parametrize("q_out,k_out,geom,refused", [
+    (1, 9, dict(qo_stride=128, qo_head_stride=64), True), (1, 9, dict(qo_stride=256, qo_head_stride=32), True),
+    (9, 2, dict(ko_stride=64, ko_head_stride=64), True), (1, 2, dict(ko_head_stride=128), True), (1, 2, dict(), False),
+    (9, 8, dict(qo_stride=128, ko_stride=64), False), (1, 2, dict(tokens=1, qo_stride=128, ko_stride=3), False)])
+def test_rope_append_in_place_needs_equal_strides(q_out, k_out, geom, refused):
+    """A thread reads both elements of a pair before it writes them, where they come from and go to the same places."""
+    strides = dict(q_stride=256, q_head_stride=64, qo_stride=256, qo_head_stride=64, k_stride=128, k_head_stride=64,
+                   ko_stride=128, ko_head_stride=64)
+    at = 4096
+    got, msg = call("nb2_rope_append", rope(**(strides | geom)), at, 2 * at, 3 * at, 4 * at, 5 * at, 6 * at, q_out * at, k_out * at,
+                    11 * at, 12 * at)
+    assert got == -1 and msg == ("RopeAppend: in place needs equal strides" if refused else "null device")
