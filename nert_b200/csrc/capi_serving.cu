@@ -201,6 +201,8 @@ int nb2_tree_attention(nb2_device* dev, const nb2_tree_attn_geom* g, const void*
         for (const void* p : {q, k_cache, v_cache, static_cast<const void*>(out)}) {
             need((reinterpret_cast<uintptr_t>(p) & 15) == 0, "TreeAttention: buffers must be 16-byte aligned");
         }
+        need(out != q || (e.o_stride == e.q_stride && e.o_head_stride == e.q_head_stride),
+             "TreeAttention: in place needs equal strides");
         bind(dev);
         tree_attention(dev, TreeAttnArgs{e, q, k_cache, v_cache, block_table, total_lens, token_offsets,
                                          reinterpret_cast<const uint32_t*>(tree_mask), out, lse, nullptr});

@@ -68,3 +68,11 @@ def test_rope_append_in_place_needs_equal_strides(q_out, k_out, geom, refused):
     got, msg = call("nb2_rope_append", rope(**(strides | geom)), at, 2 * at, 3 * at, 4 * at, 5 * at, 6 * at, q_out * at, k_out * at,
                     11 * at, 12 * at)
     assert got == -1 and msg == ("RopeAppend: in place needs equal strides" if refused else "null device")
+
+
+@pytest.mark.parametrize("geom,refused", [(dict(o_stride=512), True), (dict(o_head_stride=128), True), (dict(), False),
+                                          (dict(tokens=1, o_stride=512), False)])
+def test_tree_attention_in_place_needs_equal_strides(geom, refused):
+    """A row is written when all that read its query have; with other strides it would lie over other rows' queries."""
+    got, msg = call("nb2_tree_attention", attn(**geom), *ATTN)  # out is q there
+    assert got == -1 and msg == ("TreeAttention: in place needs equal strides" if refused else "null device")

@@ -285,3 +285,12 @@ def test_any_stride_of_a_dimension_of_one(cuda, dtype, olds, news, hq, hkv, bloc
     q1, k1 = serving.rope_append(b.q, _odd_ones(k, 0, 1), None, table, pos)
     serving.synchronize()
     assert torch.equal(q0, q1) and torch.equal(k0, k1)
+
+
+@pytest.mark.parametrize("dtype,olds,news", [("bf16", [3000, 10], [1, 1]), ("f32", [900, 40, 0], [9, 12, 3]), ("f16", [5000, 70], [64, 33])])
+def test_tree_attention_over_its_queries(cuda, dtype, olds, news):
+    b = Batch(olds, news, 8, 2, 128, 16, dtype)
+    want, want_lse = b.run()
+    out, lse = b.run(out=b.q)
+    serving.synchronize()
+    assert out.data_ptr() == b.q.data_ptr() and torch.equal(out, want) and torch.equal(lse, want_lse)
