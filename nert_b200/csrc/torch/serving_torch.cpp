@@ -324,13 +324,20 @@ std::tuple<Tensor, OptTensor> tree_attention(const Tensor& q, const Tensor& k_ca
     return {o, lse};
 }
 
+// The library takes a null list or mask for none. One that is given and holds nothing has no address of its own: it gets
+// another's, so that what points into it (offsets, rows) is checked against its count, 0, and nothing is read from it.
+template <typename T>
+const T* given(const T* p, const void* other) {
+    return p != nullptr ? p : static_cast<const T*>(other);
+}
+
 using List = std::optional<std::tuple<Tensor, Tensor>>;
 
 void list(const List& l, const char* name, c10::Device on, int64_t requests, const int32_t*& ids, const int32_t*& offsets,
           int64_t& count) {
     if (l.has_value()) {
-        ids = ints(std::get<0>(*l), name, on);
         offsets = ints(std::get<1>(*l), name, on);
+        ids = given(ints(std::get<0>(*l), name, on), offsets);
         NEED(std::get<1>(*l).size(0) == requests + 1, name, ": expected requests + 1 offsets");
         count = std::get<0>(*l).size(0);
     }
@@ -388,7 +395,7 @@ Tensor logits_process(const Tensor& logits, const List& prompt, const List& outp
     list(output, "output", on, requests, o_ids, o_off, g.output_count);
     if (bias.has_value()) {
         list(std::make_tuple(std::get<0>(*bias), std::get<2>(*bias)), "bias", on, requests, b_ids, b_off, g.bias_count);
-        b_val = floats(std::get<1>(*bias), "bias values", on, g.bias_count);
+        b_val = given(floats(std::get<1>(*bias), "bias values", on, g.bias_count), b_off);
     }
     if (grammar.has_value()) {
         const Tensor& mask = std::get<0>(*grammar);
@@ -397,7 +404,7 @@ Tensor logits_process(const Tensor& logits, const List& prompt, const List& outp
                  (mask.size(1) <= 1 || mask.stride(1) == 1) && mask.size(1) * 32 >= g.vocab,
              "grammar: expected [n, ceil(vocab / 32)] int32 words on the GPU of the others");
         NEED(!rows.has_value() || (rows->dim() == 1 && rows->size(0) == g.rows), "grammar rows: expected one a row");
-        m = static_cast<const int32_t*>(mask.data_ptr());
+        m = given(static_cast<const int32_t*>(mask.data_ptr()), logits.data_ptr());
         m_rows = ints(rows, "grammar rows", on);
         g.grammar_count = mask.size(0);
         g.grammar_stride = mask.size(0) > 1 ? mask.stride(0) : mask.size(1);

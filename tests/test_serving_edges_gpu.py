@@ -294,3 +294,20 @@ def test_tree_attention_over_its_queries(cuda, dtype, olds, news):
     out, lse = b.run(out=b.q)
     serving.synchronize()
     assert out.data_ptr() == b.q.data_ptr() and torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+def test_logit_lists_and_masks_that_hold_nothing(cuda):
+    """What points into an empty list or set of masks is checked as into any other."""
+    x = torch.randn(2, 64, device="cuda")
+    none, words = i32([]), torch.zeros(0, 2, device="cuda", dtype=torch.int32)
+    values = torch.zeros(0, device="cuda")
+    got = serving.logits_process(x, prompt=(none, i32([0, 0, 0])), output=(none, i32([0, 0, 0])),
+                                 bias=(none, values, i32([0, 0, 0])), grammar=(words, i32([-1, -1])))
+    serving.synchronize()
+    assert torch.equal(got, x)
+    for wrong in (dict(prompt=(none, i32([0, 1, 1]))), dict(output=(none, i32([0, 0, 3]))),
+                  dict(bias=(none, values, i32([0, 2, 2]))), dict(grammar=(words, i32([-1, 0]))), dict(grammar=(words, None))):
+        serving.logits_process(x, **wrong)
+        with pytest.raises(_lib.NB2Error) as e:
+            serving.synchronize()
+        assert e.value.status == _lib.ERR_DEVICE
