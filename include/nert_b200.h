@@ -373,7 +373,8 @@ int nb2_rope_append(nb2_device* dev, const nb2_rope_geom* g, const void* q, cons
  * h reading key/value head h / (q_heads/kv_heads); lse[t, h] (may be null) =
  * log sum_j exp(scale q.k_j), fp32. A token that sees nothing has out 0 and lse
  * -inf, as have tokens past token_offsets[batch]. Scores, softmax and sums in
- * fp32; NB2_F32 products by the 3xTF32 split. max_new bounds the new tokens of
+ * fp32; NB2_F32 products by the 3xTF32 split, in which values above 3.4019e38
+ * count as infinite where a token sees them. max_new bounds the new tokens of
  * a request (more are a device error, and such a request's tokens get out 0).
  * head_dim a multiple of 8 up to 256, every stride and pointer 16-byte aligned,
  * batch <= 8192, kv_heads <= 65535. Scratch comes from the device workspace. */

@@ -90,6 +90,16 @@ __device__ __forceinline__ void split_tf32(float x, float& high, float& low) {
     low = x - high;
 }
 
+// Whether 0 times x is not 0 in the products: infinities and NaN, and in float32 what split_tf32 rounds to infinity.
+template <typename T>
+__device__ __forceinline__ bool spoils(T x) {
+    if constexpr (sizeof(T) == 4) {
+        return (__float_as_uint(x) & 0x7fffffffu) + 0x1000u >= 0x7f800000u;
+    } else {
+        return !isfinite(to_f32(x));
+    }
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     if constexpr (std::is_same_v<T, __half>) {
@@ -312,7 +322,7 @@ __global__ void __launch_bounds__(32 * WR * WK, Shape<T, DP, WR, WK>::kPerSm)
             uint8_t* vt = kt + S::kTile;
             uint64_t odd = 0; // places whose values are not finite
             if (!plain) {
-                // Values that are not finite would reach the rows that do not
+                // Values that are not finite (or not in tf32) would reach the rows that do not
                 // see them as 0 * inf: taken out of the tile here, added for the rows that do below.
                 if (tid == 0) {
                     odd_keys = 0;
@@ -325,7 +335,7 @@ __global__ void __launch_bounds__(32 * WR * WK, Shape<T, DP, WR, WK>::kPerSm)
                     bool found_odd = false;
 #pragma unroll
                     for (int x = 0; x < static_cast<int>(16 / sizeof(T)); ++x) {
-                        found_odd |= !isfinite(to_f32(e[x]));
+                        found_odd |= spoils(e[x]);
                     }
                     if (found_odd) {
                         atomicOr(&odd_keys, 1ull << row);

@@ -311,3 +311,34 @@ def test_logit_lists_and_masks_that_hold_nothing(cuda):
         with pytest.raises(_lib.NB2Error) as e:
             serving.synchronize()
         assert e.value.status == _lib.ERR_DEVICE
+
+
+@pytest.mark.parametrize("val", [3.4028234663852886e38, -3.4028234663852886e38, 3.4015e38, 3.4e38])
+def test_largest_values_in_places_that_are_not_seen(cuda, val):
+    """Finite float32 values up to the largest in one drafted token's row reach the token that sees it and no others."""
+    news = [9, 40]
+    b, clean = (Batch([50, 300], news, 2, 2, 128, 16, "f32", trees="star") for _ in range(2))
+    t, r, i = 9 + 7, 1, 7
+    p = int(b.old[r]) + i
+    b.vc[int(b.table[r, p // 16]), p % 16, :, ::5] = val
+    b.kc[int(b.table[r, p // 16]), p % 16, 1, 3] = val
+    out, lse = b.run()
+    want, want_lse = clean.run()
+    serving.synchronize()
+    rest = [x for x in range(out.shape[0]) if x != t]
+    assert torch.equal(out[rest], want[rest]) and torch.equal(lse[rest], want_lse[rest])
+    # the token that sees it: its weight (head 0, whose key is as it was) times the value and the sum of the others
+    q, k = b.q[t, 0].double().cpu().numpy(), b.k[r][:, 0]
+    see = np.arange(int(b.total[r])) < int(b.old[r])
+    see[p] = True
+    s = np.where(see, k @ q * b.scale, -np.inf)
+    w = np.exp(s - s.max())
+    w /= w.sum()
+    got = out[t, 0].double().cpu().numpy()
+    wanted = w @ b.v[r][:, 0]
+    wanted[::5] += w[p] * (val - b.v[r][p, 0, ::5])
+    assert np.isfinite(got).all()
+    # scores and sums as in Batch.check; its largest value is the planted one in those columns
+    most = np.where(np.arange(128) % 5 == 0, abs(val) * w[p] + 10, 10)
+    eps = 2 * (128 + 16) * 2.0**-23 * (np.abs(k) @ np.abs(q))[see].max() * b.scale + (int(b.total[r]) + 64) * 2.0**-23 + 2.0**-20
+    assert (np.abs(got - wanted) <= (eps + 4 * 2.0**-24) * most).all()
