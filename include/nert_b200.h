@@ -93,14 +93,14 @@ int nb2_device_open(int ordinal, nb2_device** out);
  * device error word of its own: work of this context is ordered with the
  * caller's other work on that stream, and contexts of different streams share
  * no scratch. The stream must outlive the context. Any row takes it in place of
- * nb2_device_open's. One host thread at a time per context. A call makes the
- * context's GPU current for its thread. The caller may
- * capture the stream in a CUDA graph once the context is made: the graph then
- * has a workspace of its own (up to 39 MB, taken back when the graph and its
- * executable are gone) and may be replayed on any stream beside other work; two
- * executables made of one graph share it and may not run at once. Device errors
- * of replayed graphs are kept by GPU: the next synchronisation of any context of
- * this kind reports them. */
+ * nb2_device_open's. One host thread at a time per context (but several may be
+ * in nb2_device_synchronize); a call makes the context's GPU current for its
+ * thread. The caller may capture the stream in a CUDA graph once the context is
+ * made: the graph then has a workspace of its own (up to 40 MB, taken back when
+ * the graph and its executable are gone) and may be replayed on any stream beside
+ * other work; two executables made of one graph share it and may not run at once.
+ * Device errors of replayed graphs are kept by GPU: the next synchronisation of
+ * any context of this kind reports them. */
 int nb2_device_on_stream(int ordinal, void* stream, nb2_device** out);
 /* Waits for the stream, then frees a context from nb2_device_on_stream (null
  * is a no-op; a context from nb2_device_open is NB2_ERR_INVALID). */
@@ -372,12 +372,15 @@ int nb2_rope_append(nb2_device* dev, const nb2_rope_geom* g, const void* q, cons
  * tree_mask: j <= i). out[t, h] = sum_j softmax_j(scale q.k_j) v_j with query head
  * h reading key/value head h / (q_heads/kv_heads); lse[t, h] (may be null) =
  * log sum_j exp(scale q.k_j), fp32. A token that sees nothing has out 0 and lse
- * -inf, as have tokens past token_offsets[batch]. Scores, softmax and sums in
- * fp32; NB2_F32 products by the 3xTF32 split, in which values above 3.4019e38
- * count as infinite where a token sees them. max_new bounds the new tokens of
- * a request (more are a device error, and such a request's tokens get out 0).
- * head_dim a multiple of 8 up to 256, every stride and pointer 16-byte aligned,
- * batch <= 8192, kv_heads <= 65535. Scratch comes from the device workspace. */
+ * -inf, as have tokens past token_offsets[batch]. out may be q (same strides).
+ * Scores, softmax and sums in fp32; 16-bit weights are rounded to the cache's
+ * type for their product with v (not for their sum). NB2_F32 products by the
+ * 3xTF32 split, in which values above 3.4019e38 count as infinite where a token
+ * sees them. max_new bounds the new tokens of a request (more are a device
+ * error, and such a request's tokens get out 0) and picks the kernel and its
+ * blocks of rows: far above the real number it costs time. head_dim a multiple
+ * of 8 up to 256, every pointer and the stride of every dimension of more than
+ * one 16-byte aligned, batch <= 8192, kv_heads <= 65535. Scratch comes from the device workspace. */
 typedef struct nb2_tree_attn_geom {
     int64_t batch, tokens, q_heads, kv_heads, head_dim, max_new;
     int64_t q_stride, q_head_stride, o_stride, o_head_stride;
@@ -394,7 +397,7 @@ int nb2_tree_attention(nb2_device* dev, const nb2_tree_attn_geom* g, const void*
 
 /* Logit rules: for row i with request r = row_request[i] (null: r = i) and
  * token v, c = how often v is in the request's output list, and seen = c > 0 or
- * v in its prompt list, in fp32:
+ * v in its prompt list, in fp32 (the division as a product with 1 / repetition):
  *   x = logits[i, v];  seen: x = x > 0 ? x / repetition[r] : x * repetition[r];
  *   x -= frequency[r] * c + (c > 0 ? presence[r] : 0);  x += bias[r, v];
  *   x = -inf where grammar row grammar_rows[i] (null: i; negative: no rule) has

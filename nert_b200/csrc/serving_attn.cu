@@ -26,7 +26,9 @@
 // Measured: 4 single tokens over 60-2,000 places, 32/8 heads of 128 in bfloat16 (16 MB): 16 us, bound by latencies (of 29,000
 // clocks with cold caches the lengths take 3,000, q 2,400, the first tile 5,000, the join 10,000). 8 trees of 5-24
 // tokens over 100-3,000 places, 12 heads of 64 in float32 (76 MB): 55 us, 1.4 TB/s, bound by the three tf32 products of
-// each product and their operands' splits at one CTA an SM (233 registers).
+// each product and their operands' splits at one CTA an SM (233 registers). Heads of more than 128 elements do not fit
+// 255 registers: 560-732 bytes a thread are spilled in 16-bit types, 208-232 in float32 (64-element heads in blocks of 32 rows
+// spill 192, to leave an SM two CTAs; the rest at most 48).
 
 #include "serving_attn.cuh"
 

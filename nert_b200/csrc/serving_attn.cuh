@@ -320,8 +320,8 @@ __device__ __forceinline__ Span find_span(const TreeAttnArgs& a, int group, int 
 // An item's pieces are joined by one CTA when it has a few; where few items share the GPU (one long context), each is in
 // many, which that CTA reads one after another while the others are gone: then a second launch joins them, a slice
 // of an item's elements a CTA. By the CTA / by the launch, bfloat16, 60,000 places: 64 tokens, 32/8 heads of 128 (18 pieces
-// of 128 KB) 119 / 99 us, 8/1 heads (74 pieces) 154 / 58; 8 tokens, 32/8 heads (18 of 16 KB) 96 / 93; 8,000 places, 33 tokens 66 / 40.
-// One token (37 of 2 KB) takes 59 us and 57 with no join at all, so nothing would be gained there.
+// of 128 KB) 123 / 99 us, 8/1 heads (74 pieces) 152 / 58; 8 tokens, 32/8 heads (18 of 16 KB) 96 / 93; 8,000 places, 33 tokens 57 / 40.
+// One token (37 of 2 KB) takes 61 us and 57 with no join at all, so nothing would be gained there.
 constexpr int kJoinThreads = 256;
 constexpr int64_t kJoinApart = 256 << 10; // bytes of an item's pieces from which on that is faster
 

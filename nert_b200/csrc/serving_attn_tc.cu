@@ -18,10 +18,11 @@
 // was set (the weights and sums stay far inside the range of their types; the final division takes the reference out).
 //
 // Measured, bfloat16, head dimension 128: 16 trees of 33-64 tokens, 32/8 heads, over 300-6,000 places (216 MB) 90 us, 2.4 TB/s
-// and 470 TFLOP/s; 8 of 7-16 tokens, 40/8 heads, over 9,000-60,000 places (1.1 GB, float16) 207 us, 5.4 TB/s, bound by HBM. The
-// first is bound by a tile's chain of copy, scores, softmax and products (4,450 clocks, where HBM alone takes 2,800) and
+// and 470 TFLOP/s; 8 of 7-16 tokens, 40/8 heads, over 9,000-60,000 places (1.1 GB, float16) 235 us among other passes
+// (4.7 TB/s; 207 us and 5.4 TB/s with an idle GPU before it), bound by HBM but for item ends. The first is bound by a tile's chain of copy, scores, softmax and products (4,450 clocks, where HBM alone takes 2,800) and
 // by what a CTA does before its first tile (20,000 clocks) and after its last (16,000, with a join). Whole tiles
 // of scores in place of halves 98 us; both slabs of a page as one 5-D box 2 us more on the first, 4 less on the second.
+// ptxas spills 194-202 bytes a thread in each instance (what lives across the items, under the launch's 168 registers).
 //
 // Values that are not finite, and rows past the end of a page list, would reach rows that do not see them
 // as 0 * inf: in the tiles that hold new tokens (or holes) the group clears such rows of V in shared
@@ -142,7 +143,7 @@ __device__ __forceinline__ void tma_load_page(void* dst, const CUtensorMap* map,
                  : "memory");
 }
 
-// Registers of a warp group: the launch's 168 x 384 go as 208 to each softmax group (a row's 128 scores stay in
+// Registers of a warp group: the launch's 168 x 384 go as 208 to each softmax group (half a row's scores, 64, stay in
 // registers) and 88 to the third.
 template <int N>
 __device__ __forceinline__ void regs_up() {
@@ -616,7 +617,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     __syncwarp();
                     tc_fence_after();
                     float zz[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    // 32 scores to weights, packed over the scores; their sum keeps all bits
+                    // 32 scores to weights, packed over the scores. They are rounded to the cache's type, as both operands of
+                    // the product must have it: each at most u off, which the sum over places averages (the error against
+                    // 64 bits is 1.1 to 1.4 times that of unrounded weights; a second product of their rest would double
+                    // the tensor cores' work). The sum z keeps all their bits.
                     auto weights = [&](int c, const float* x, float ref) {
                         uint32_t pk[16];
 #pragma unroll
@@ -964,8 +968,8 @@ bool tree_attention_tc_takes(const TreeAttnArgs& a, int sms) {
                       g.vc_head_stride}) {
         strides = strides && s > 0 && s < most;
     }
-    // Up to 64 rows with less than a tile a CTA: an item's beginning and end cost more than its products (2 requests of
-    // 48 rows over 3,400 places 40 us here, 22 us there; 7 of them over 3,000 places 31 and 51 us).
+    // Up to 64 rows with less than a tile a CTA: an item's beginning and end cost more than its products (48 rows, 2 key/value
+    // heads: 2 requests over 3,400 places 34 us here and 26 there, 7 over 3,000 places 31 and 39; 8 heads 45 and 59).
     const int64_t tiles = g.batch * g.kv_heads * ((g.table_blocks * g.block_size + kTile - 1) / kTile);
     const bool enough = rows > 64 || (rows > kTcRows && tiles > sms);
     return g.dtype != kF32 && enough && g.head_dim >= 64 && g.head_dim <= 128 && page && strides && g.num_blocks > 0;

@@ -15,9 +15,10 @@
 // every row of the request is streamed, the next row's loads in flight, every element through the same
 // few instructions: x * (x > 0 ? 1/rep : rep or 1) + word.
 // Measured (408 rows of 128,000 tokens in bfloat16 to float32, 313 MB, 24 requests of up to 8,000
-// tokens): 82 us, 3.9 TB/s. Rules only where a bitmap has a bit, inside the stream (some lane of nearly every warp
+// tokens): 84 us among other passes, 3.8 TB/s. Rules only where a bitmap has a bit, inside the stream (some lane of nearly every warp
 // has one; 37 instructions an element): 115 us. Plain stream, then single stores at the touched
-// tokens (each a read and a partial write of a sector in L2): 150 us.
+// tokens (each a read and a partial write of a sector in L2): 150 us. Five CTAs an SM leave 48 registers, which suit
+// 16-bit logits; the float32 forms spill 80 bytes a thread there.
 
 #include "serving.cuh"
 

@@ -16,6 +16,10 @@ token ids) are checked by the kernels, and ``synchronize()`` raises what they
 recorded. The checks and the call run in nert_b200_torch.so
 (``csrc/torch/serving_torch.cpp``); there is no fallback without it.
 
+Inference only: outputs carry no gradient, whatever the inputs ask for. The
+context of a stream is kept for the life of the process, with its workspace (up
+to 40 MB, outside torch's allocator); torch's streams come from fixed pools.
+
 Metadata tensors are contiguous int32; masks are int32 words of 32 bits.
 """
 
@@ -130,7 +134,8 @@ def tree_attention(q, k_cache, v_cache, block_table, seq_lens, token_offsets, tr
     [batch + 1] and ``tree_mask`` [tokens, words] as ``page_plan`` gives them. A
     new token sees every older place of its request and the new ones in its mask
     row; without a mask, the new ones up to itself. ``max_new`` bounds the new
-    tokens of a request (default: all of them). ``scale`` defaults to
+    tokens of a request (default: all of them) and picks the kernel: give it,
+    where a call has many requests of few tokens. ``scale`` defaults to
     head_dim ** -0.5. Returns out, or (out, lse) with lse [tokens, q_heads] float32.
     A token that sees nothing has out 0 and lse -inf.
     """
