@@ -147,6 +147,45 @@ def test_graphs_of_one_stream_replayed_at_once(cuda, dtype, olds, news):
         serving.synchronize()
 
 
+def test_graphs_of_a_split_contraction_replayed_at_once(cuda):
+    """Any row of the library on a caller's stream: here the partial sums of a Gemm that splits its long side."""
+    from nert_b200._lib import check, ctypes, lib
+
+    rows, n, k = 64, 64, 16384
+    ws = [torch.randn(n, k, device="cuda") for _ in range(2)]
+    xs = [torch.randn(rows, k, device="cuda") for _ in range(2)]
+
+    def gemm(x, packed, y):
+        check(lib().nb2_gemm_run_packed(serving.context(), x.data_ptr(), packed.data_ptr(), None, 0, y.data_ptr(), rows, n, k, 0,
+                                        1.0, 1.0, _lib.ACT_NONE))
+        return y
+
+    packs = []
+    for w in ws:
+        size = ctypes.c_int64()
+        check(lib().nb2_gemm_packed_size(n, k, ctypes.byref(size)))
+        packs.append(torch.empty(size.value, device="cuda", dtype=torch.uint8))
+        check(lib().nb2_gemm_pack(serving.context(), w.data_ptr(), n, k, 1, packs[-1].data_ptr()))
+    ys = [torch.empty(rows, n, device="cuda") for _ in range(2)]
+    want = [gemm(x, p, torch.empty_like(ys[0])) for x, p in zip(xs, packs)]
+    slices = ctypes.c_int()
+    check(lib().nb2_device_last_contraction(serving.context(), None, None, ctypes.byref(slices), None, None))
+    assert slices.value > 1
+    serving.synchronize()
+    first, others = torch.cuda.Stream(), [torch.cuda.Stream() for _ in range(2)]
+    graphs = [_in_graph(first, lambda x=x, p=p, y=y: gemm(x, p, y), 20)[0] for x, p, y in zip(xs, packs, ys)]
+    for _ in range(10):
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, others):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, w) for y, w in zip(ys, want))
+    for y, x, w in zip(ys, xs, ws):
+        ref = x.double() @ w.double().T
+        assert ((y.double() - ref).abs().max() / ref.abs().max()).item() <= 1e-4
+
+
 def test_graphs_give_their_workspace_back(cuda):
     """A workspace belongs to a graph as long as it lives: the next capture takes one that a dead graph had."""
     b = Batch([30000], [12], 4, 1, 128, 16, "bf16")
